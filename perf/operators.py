@@ -224,7 +224,8 @@ def _quantise(x):
     x = x.float()
     head = x.shape[-1]
     m = x.amin(-1).bfloat16()
-    s = ((x.amax(-1) - m.float()).clamp_min(0) / 15).bfloat16()
+    fifteen = x.new_full((), 15.0)  # a tensor: torch multiplies by the reciprocal of a number
+    s = ((x.amax(-1) - m.float()).clamp_min(0) / fifteen).bfloat16()
     bad = ~(torch.isfinite(m) & torch.isfinite(s) & torch.isfinite(x).all(-1))
     m, s = m.masked_fill(bad, math.nan), s.masked_fill(bad, math.nan)
     # 64 bits: a quotient next to a half has to fall on its own side
