@@ -423,6 +423,53 @@ class KvCache:
 
 
 @dataclass
+class Kv4Layer:
+    """One layer of a 4-bit key/value cache: uint32 codes [(batch,) kv_heads, seq, words] and
+    scales [(batch,) kv_heads, seq] for keys and values (format: ab_kv4_layer in the header)."""
+    key_codes: Tensor
+    key_scales: Tensor
+    value_codes: Tensor
+    value_scales: Tensor
+
+    @property
+    def c(self) -> _abi.Kv4Layer_t:
+        return _abi.Kv4Layer_t(self.key_codes.t, self.key_scales.t, self.value_codes.t,
+                               self.value_scales.t)
+
+
+class Kv4Cache:
+    """Persistent 4-bit key/value cache of (batch) streams, beside KvCache: about 0.53 bytes a
+    value at head 128 where f32 takes 4 and bf16 2."""
+
+    def __init__(self, rt: Runtime, layers, seq_len, kv_heads, head_size, batch=1):
+        h = C.c_void_p()
+        _check(_abi.lib().ab_kv4cache_create(rt.handle, layers, seq_len, kv_heads, head_size,
+                                             batch, C.byref(h)))
+        self._h = h
+        self.rt = rt
+
+    def layer(self, layer: int) -> Kv4Layer:
+        c = _abi.Kv4Layer_t()
+        _check(_abi.lib().ab_kv4cache_layer(self._h, layer, C.byref(c)))
+        return Kv4Layer(*[Tensor(t, self.rt, owner=self) for t in
+                          (c.key_codes, c.key_scales, c.value_codes, c.value_scales)])
+
+    def zero(self):
+        _check(_abi.lib().ab_kv4cache_zero(self._h))
+
+    def close(self):
+        if getattr(self, "_h", None):
+            _abi.lib().ab_kv4cache_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+@dataclass
 class CausalAttentionBlockWeights:
     norm: Tensor
     query: Tensor
@@ -849,7 +896,7 @@ from . import kernels  # noqa: E402  (the reference's kernel-level API)
 __all__ = [
     "AmmonError", "ValidationError", "DeviceError", "Runtime", "create_runtime", "Tensor",
     "DecodeStep", "Scheme", "Embedding", "RmsNorm", "Linear", "KvCache", "KvLayer",
-    "CausalAttentionBlock", "CausalAttentionBlockWeights", "SwiGluBlock",
+    "Kv4Cache", "Kv4Layer", "CausalAttentionBlock", "CausalAttentionBlockWeights", "SwiGluBlock",
     "SwiGluBlockWeights", "LlamaConfig", "LlamaModel", "Comm", "AutoregressiveModel",
     "generate_tokens", "generate", "GenerateOptions", "GenerateOutput", "GenerateTokenOutput",
     "sample_argmax", "BpeTokenizer", "NativeBpeTokenizer", "Tokenizer", "kernels",

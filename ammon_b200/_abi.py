@@ -39,6 +39,11 @@ class SwigluWeights_t(C.Structure):
     _fields_ = [("norm", Tensor_t), ("gate", Tensor_t), ("up", Tensor_t), ("down", Tensor_t)]
 
 
+class Kv4Layer_t(C.Structure):
+    _fields_ = [("key_codes", Tensor_t), ("key_scales", Tensor_t), ("value_codes", Tensor_t),
+                ("value_scales", Tensor_t)]
+
+
 class LlamaConfig_t(C.Structure):
     _fields_ = [("dim", C.c_uint32), ("layers", C.c_uint32), ("heads", C.c_uint32),
                 ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("hidden", C.c_uint32),
@@ -112,6 +117,13 @@ SIGNATURES = {
     "ab_kvcache_layer": (C.c_int, [P, u32, C.POINTER(T), C.POINTER(T)]),
     "ab_kvcache_zero": (C.c_int, [P]),
     "ab_kvcache_destroy": (C.c_int, [P]),
+    "ab_kv4cache_create": (C.c_int, [P, u32, u32, u32, u32, u32, PP]),
+    "ab_kv4cache_layer": (C.c_int, [P, u32, C.POINTER(Kv4Layer_t)]),
+    "ab_kv4cache_zero": (C.c_int, [P]),
+    "ab_kv4cache_destroy": (C.c_int, [P]),
+    "ab_kernel_kv4_store": (C.c_int, [P, T, T, C.POINTER(Kv4Layer_t), T]),
+    "ab_kernel_kv4_load": (C.c_int, [P, C.POINTER(Kv4Layer_t), T, T, T]),
+    "ab_kernel_kv4_attention": (C.c_int, [P, T, C.POINTER(Kv4Layer_t), T, T]),
     "ab_attention_block_create": (C.c_int, [P, u32, u32, u32, u32, f32, PP]),
     "ab_attention_block_record": (C.c_int, [P, P, T, C.POINTER(AttentionWeights_t), T, T, T]),
     "ab_attention_block_destroy": (C.c_int, [P]),

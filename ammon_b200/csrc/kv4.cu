@@ -1,0 +1,480 @@
+// The 4-bit key/value cache: quantising rows as they are written, reading rows back, and the
+// cache handle. Attention over it is in kv4_attention.cu.
+//
+// One vector is what one kv head keeps for one position: `head` values, held as 4-bit codes and
+// one word with two bf16 numbers, the step s (low half) and the offset m (high half):
+//     m = bf16(min x)   s = bf16(max(max x - m, 0) / 15)   c_i = rne((x_i - m) / s) in 0..15
+// and standing for m + s c_i. A vector with a value that is not finite, or whose range is not,
+// has NaN for both and reads back as NaN throughout. Element i is bits 4 (i % 8) and up of word
+// i / 8; a row of codes is padded with zeros to a multiple of 16 bytes (32 elements). Arrays are
+// head-major ([batch,] kv_heads, seq, words), so that the positions of one head are one
+// contiguous run for the attention that streams them.
+#include <algorithm>
+#include <string>
+
+#include "common.cuh"
+#include "internal.h"
+#include "kv4.h"
+
+namespace ab {
+
+// ---- operands ---------------------------------------------------------------------------
+Kv4View kv4_operands(const ab_kv4_layer& c, uint32_t rows, uint32_t kv_heads, uint32_t head) {
+    static const char* names[4] = {"cache.key_codes", "cache.key_scales", "cache.value_codes",
+                                   "cache.value_scales"};
+    const ab_tensor t[4] = {c.key_codes, c.key_scales, c.value_codes, c.value_scales};
+    for (int i = 0; i < 4; i++) {
+        expect_data(names[i], t[i]);
+        expect_dtype(names[i], t[i], AB_U32);
+    }
+    if (head == 0 || head > kKv4MaxHead)
+        invalid("kv4: head size " + std::to_string(head) + " is not in 1..128");
+    expect_rank_in(names[0], t[0], 3, 4);
+    const int cr = t[0].rank;
+    for (int i = 0; i < 4; i++) {
+        expect_rank(names[i], t[i], i % 2 ? cr - 1 : cr);
+        for (int a = 0; a < t[i].rank; a++)
+            if (t[i].dims[a] != t[0].dims[a])
+                invalid(std::string("parameter `") + names[i] +
+                        "`: leading dims must match cache.key_codes " + shape_str(t[0]));
+    }
+    if (cr == 4 && t[0].dims[0] < rows) expect_dim(names[0], t[0], 0, "batch", rows);
+    expect_dim(names[0], t[0], cr - 3, "kv_heads", kv_heads);
+    expect_dim(names[0], t[0], cr - 1, "words", kv4_words(head));
+    for (int i = 0; i < 4; i++)
+        if ((uintptr_t)t[i].data % (i % 2 ? 4 : 16))
+            invalid(std::string("parameter `") + names[i] + "`: must be " +
+                    (i % 2 ? "4" : "16") + "-byte aligned");
+    Kv4View v = {};
+    v.kv_heads = kv_heads;
+    v.head = head;
+    v.seq = t[0].dims[cr - 2];
+    v.words = t[0].dims[cr - 1];
+    v.row_stride = cr == 4 ? (uint64_t)kv_heads * v.seq : 0;
+    for (int w = 0; w < 2; w++) {
+        v.codes[w] = (uint32_t*)t[2 * w].data;
+        v.scales[w] = (uint32_t*)t[2 * w + 1].data;
+    }
+    return v;
+}
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kUnroll = 4;  // vectors a lane group has in flight
+
+// 16 bytes that are read once. Not the non-coherent path: this grid may have started while the
+// kernel that writes them still ran.
+__device__ __forceinline__ uint4 ld_once(const void* p) {
+    uint4 r;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+                 : "l"(p));
+    return r;
+}
+
+// Eight elements of a row from element e on (`left` of them exist; vec: 16-byte loads).
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, uint32_t left, bool vec, float* v) {
+    if (vec && left >= 8) {
+        if constexpr (sizeof(T) == 2) {
+            const uint4 r = ld_once(p);
+            v[0] = bf16lo(r.x); v[1] = bf16hi(r.x); v[2] = bf16lo(r.y); v[3] = bf16hi(r.y);
+            v[4] = bf16lo(r.z); v[5] = bf16hi(r.z); v[6] = bf16lo(r.w); v[7] = bf16hi(r.w);
+        } else {
+            const uint4 a = ld_once(p), b = ld_once(p + 4);
+            v[0] = __uint_as_float(a.x); v[1] = __uint_as_float(a.y);
+            v[2] = __uint_as_float(a.z); v[3] = __uint_as_float(a.w);
+            v[4] = __uint_as_float(b.x); v[5] = __uint_as_float(b.y);
+            v[6] = __uint_as_float(b.z); v[7] = __uint_as_float(b.w);
+        }
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) v[i] = i < left ? to_f32(p[i]) : 0.0f;
+    }
+}
+
+// The code of x: the whole number nearest to (x - m) / s in real arithmetic, halves to even,
+// within 0..15. u = fl(fl(x - m) * fl(1 / s)) is within 3 * 2^-24 * 16 < 3e-6 of the quotient
+// wherever |u| <= 16, so it decides every case but those within 1e-5 of a half; these, and
+// steps whose reciprocal is not a normal number, take the quotient in 64 bits.
+__device__ __forceinline__ uint32_t code_of(float x, float m, float s, float inv) {
+    const float u = fminf(fmaxf((x - m) * inv, -1.0f), 16.0f);
+    const float k = rintf(u);
+    if (fabsf(u - k) < 0.49999f && inv < 1e37f) return (uint32_t)fminf(fmaxf(k, 0.0f), 15.0f);
+    const double q = ((double)x - (double)m) / (double)s;
+    return (uint32_t)fmin(fmax(rint(q), 0.0), 15.0);
+}
+
+constexpr uint32_t kRowsPerScan = 1024;
+
+// ordered[i]: the rows [1024 i, 1024 (i + 1)] of the parcel are at strictly rising positions.
+__global__ void __launch_bounds__(kRowsPerScan)
+    kv4_order_kernel(const Step* step, uint32_t rows, uint32_t* ordered) {
+    pdl_wait();
+    pdl_trigger();
+    const uint32_t r = blockIdx.x * kRowsPerScan + threadIdx.x;
+    const bool ok = r + 1 >= rows || step[r].position < step[r + 1].position;
+    const int all = __syncthreads_and(ok);
+    if (threadIdx.x == 0) ordered[blockIdx.x] = all;
+}
+
+// LPV lanes hold one vector, eight elements (one code word) each; a block takes kUnroll *
+// kThreads / LPV consecutive vectors of one of the two tensors (blockIdx.y), kv heads fastest,
+// so its loads are one contiguous run of the source. All of a lane's loads are issued before
+// the first is used.
+template <typename T, int LPV>
+__global__ void __launch_bounds__(kThreads)
+    kv4_store_kernel(const T* key, const T* value, const Kv4View c,
+                     uint32_t rows, const Step* step, int vec,
+                     const uint32_t* ordered, uint32_t* flags) {
+    constexpr uint32_t GROUPS = kThreads / LPV;
+    constexpr uint32_t VECS = GROUPS * kUnroll;
+    __shared__ uint32_t lost[VECS];  // per row of this block: a later row has its position
+    pdl_wait();
+    const uint32_t which = blockIdx.y;
+    const T* src = which ? value : key;
+    const uint64_t total = (uint64_t)rows * c.kv_heads;
+    const uint64_t v0 = (uint64_t)blockIdx.x * VECS;
+    const uint32_t sub = threadIdx.x % LPV, grp = threadIdx.x / LPV;
+    const uint32_t e0 = sub * 8;
+    const uint32_t left = e0 < c.head ? c.head - e0 : 0;
+    float x[kUnroll][8];
+    uint32_t row[kUnroll], kvh[kUnroll], pos[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; u++) {
+        const uint64_t v = v0 + u * GROUPS + grp;
+        const bool live = v < total;
+        row[u] = live ? (uint32_t)(v / c.kv_heads) : 0;
+        kvh[u] = live ? (uint32_t)(v % c.kv_heads) : 0;
+        pos[u] = live ? step[row[u]].position : 0xffffffffu;
+        load8(src + (live ? v * c.head + e0 : 0), live ? left : 0, vec, x[u]);
+        if (live && pos[u] >= c.seq && sub == 0) atomicOr(flags, kFlagPositionRange);
+    }
+    // rows of one cache at the same position: the last one is written. Rising positions (a
+    // prompt) cannot meet; otherwise the block looks through the rows after its own.
+    bool scan = c.row_stride == 0 && rows > 1;
+    if (scan && ordered) {
+        bool ok = true;
+        for (uint32_t i = threadIdx.x; i < (rows + kRowsPerScan - 1) / kRowsPerScan; i += kThreads)
+            ok = ok && ordered[i] != 0;
+        scan = !__syncthreads_and(ok);
+    }
+    if (scan) {
+        const uint32_t r0 = (uint32_t)(v0 / c.kv_heads);
+        const uint32_t r1 = (uint32_t)min((uint64_t)rows, (v0 + VECS - 1) / c.kv_heads + 1);
+        for (uint32_t r = threadIdx.x; r < VECS; r += kThreads) lost[r] = 0;
+        __syncthreads();
+        for (uint32_t q = r0 + 1 + threadIdx.x; q < rows; q += kThreads) {
+            const uint32_t pq = step[q].position;
+            for (uint32_t r = r0; r < min(q, r1); r++)
+                if (step[r].position == pq) lost[r - r0] = 1;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < kUnroll; u++)
+            if (row[u] >= r0 && row[u] < r1 && lost[row[u] - r0]) pos[u] = 0xffffffffu;
+    }
+    pdl_trigger();
+#pragma unroll
+    for (int u = 0; u < kUnroll; u++) {
+        float lo = INFINITY, hi = -INFINITY, fin = 0.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {
+            if (i < left) {
+                lo = fminf(lo, x[u][i]);
+                hi = fmaxf(hi, x[u][i]);
+                fin = fmaf(x[u][i], 0.0f, fin);  // NaN once a value is not finite
+            }
+        }
+#pragma unroll
+        for (int o = LPV / 2; o > 0; o >>= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            fin += __shfl_xor_sync(0xffffffffu, fin, o);
+        }
+        const bf16 mb = __float2bfloat16_rn(lo);
+        const float m = __bfloat162float(mb);
+        const bf16 sb = __float2bfloat16_rn(__fdiv_rn(fmaxf(__fsub_rn(hi, m), 0.0f), 15.0f));
+        const float s = __bfloat162float(sb);
+        const bool bad = !(fin == 0.0f) || !isfinite(m) || !isfinite(s);
+        uint32_t word = 0;
+        if (!bad && s > 0.0f) {
+            const float inv = 1.0f / s;
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++)
+                if (i < left) word |= code_of(x[u][i], m, s, inv) << (4 * i);
+        }
+        if (pos[u] >= c.seq) continue;
+        const uint64_t at = (uint64_t)row[u] * c.row_stride + (uint64_t)kvh[u] * c.seq + pos[u];
+        if (sub < c.words) c.codes[which][at * c.words + sub] = word;
+        if (sub == 0)
+            c.scales[which][at] = bad ? 0x7fff7fffu
+                                      : (uint32_t)__bfloat16_as_ushort(sb) |
+                                            ((uint32_t)__bfloat16_as_ushort(mb) << 16);
+    }
+}
+
+// Reading back: the same lane groups, each lane turning one code word into eight values.
+// Output row i of batch row b is position step[b].position + i; positions past the cache's
+// end give zeros and raise the position flag.
+template <typename T, int LPV>
+__global__ void __launch_bounds__(kThreads)
+    kv4_load_kernel(T* key, T* value, const Kv4View c, uint32_t batch, uint32_t n,
+                    const Step* step, int vec, uint32_t* flags) {
+    constexpr uint32_t GROUPS = kThreads / LPV;
+    constexpr uint32_t VECS = GROUPS * kUnroll;
+    pdl_wait();
+    pdl_trigger();
+    const uint32_t which = blockIdx.y;
+    T* dst = which ? value : key;
+    const uint64_t total = (uint64_t)batch * n * c.kv_heads;
+    const uint32_t sub = threadIdx.x % LPV, grp = threadIdx.x / LPV;
+    const uint32_t e0 = sub * 8;
+    uint32_t word[kUnroll], sc[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; u++) {
+        const uint64_t v = (uint64_t)blockIdx.x * VECS + u * GROUPS + grp;
+        word[u] = sc[u] = 0;
+        if (v < total) {
+            const uint64_t line = v / c.kv_heads;
+            const uint32_t kvh = (uint32_t)(v % c.kv_heads);
+            const uint32_t b = (uint32_t)(line / n);
+            const uint64_t pos = (uint64_t)step[b].position + line % n;
+            if (pos < c.seq) {
+                const uint64_t at = (uint64_t)b * c.row_stride + (uint64_t)kvh * c.seq + pos;
+                if (sub < c.words) word[u] = __ldcg(c.codes[which] + at * c.words + sub);
+                sc[u] = __ldcg(c.scales[which] + at);
+            } else if (sub == 0) {
+                atomicOr(flags, kFlagPositionRange);
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; u++) {
+        const uint64_t v = (uint64_t)blockIdx.x * VECS + u * GROUPS + grp;
+        if (v >= total || e0 >= c.head) continue;
+        const float s = bf16lo(sc[u]), m = bf16hi(sc[u]);
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = fmaf((float)((word[u] >> (4 * i)) & 15u), s, m);
+        T* p = dst + v * c.head + e0;
+        if (vec) {
+            if constexpr (sizeof(T) == 2) {
+                uint4 r;
+                __nv_bfloat162 h;
+                h = __floats2bfloat162_rn(x[0], x[1]); r.x = *reinterpret_cast<uint32_t*>(&h);
+                h = __floats2bfloat162_rn(x[2], x[3]); r.y = *reinterpret_cast<uint32_t*>(&h);
+                h = __floats2bfloat162_rn(x[4], x[5]); r.z = *reinterpret_cast<uint32_t*>(&h);
+                h = __floats2bfloat162_rn(x[6], x[7]); r.w = *reinterpret_cast<uint32_t*>(&h);
+                *reinterpret_cast<uint4*>(p) = r;
+            } else {
+                reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+                reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+            }
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++)
+                if (e0 + i < c.head) p[i] = from_f32<T>(x[i]);
+        }
+    }
+}
+
+// Rows [n, kv_heads, head], or [kv_heads, head] for one; both tensors alike.
+struct Kv4Rows {
+    uint32_t rows, kv_heads, head;
+    int vec;  // 16-byte accesses: whole groups of eight elements, aligned
+};
+
+Kv4Rows rows_of(const ab_tensor& key, const ab_tensor& value, int rank_lo, int rank_hi) {
+    expect_data("key", key);
+    expect_data("value", value);
+    expect_float("key", key);
+    expect_dtype("value", value, key.dtype);
+    expect_rank_in("key", key, rank_lo, rank_hi);
+    expect_rank("value", value, key.rank);
+    for (int a = 0; a < key.rank; a++)
+        if (value.dims[a] != key.dims[a])
+            invalid("parameter `value`: dims must match key " + shape_str(key));
+    Kv4Rows r = {};
+    r.head = key.dims[key.rank - 1];
+    r.kv_heads = key.dims[key.rank - 2];
+    const uint64_t rows = numel(key) / ((uint64_t)r.head * r.kv_heads);
+    if (rows > 0x7fffffffu) invalid("parameter `key`: too many rows");
+    r.rows = (uint32_t)rows;
+    r.vec = r.head % 8 == 0 && ((uintptr_t)key.data | (uintptr_t)value.data) % 16 == 0;
+    return r;
+}
+
+template <typename F>
+void with_lanes(uint32_t words, F&& f) {
+    if (words <= 4) f(std::integral_constant<int, 4>());
+    else if (words <= 8) f(std::integral_constant<int, 8>());
+    else f(std::integral_constant<int, 16>());
+}
+
+unsigned blocks_for(uint64_t vectors, int lanes) {
+    const uint64_t per = (uint64_t)kThreads / lanes * kUnroll;
+    const uint64_t n = (vectors + per - 1) / per;
+    if (n > 0x7fffffffu) invalid("kv4: too many vectors for one call");
+    return (unsigned)n;
+}
+
+}  // namespace
+
+void record_kv4_store(ab_scheme* s, const char* label, ab_tensor key, ab_tensor value,
+                      const ab_kv4_layer& cache, ab_tensor step) {
+    const Kv4Rows r = rows_of(key, value, 2, 3);
+    const Kv4View c = kv4_operands(cache, r.rows, r.kv_heads, r.head);
+    expect_step(step, r.rows);
+    const Step* st = (const Step*)step.data;
+    uint32_t* flags = s->rt ? s->rt->flags : nullptr;
+    // Rows over one cache: every block looks for later rows at its rows' positions. Where that
+    // takes a thread more than 512 comparisons (about 1 us), whether the positions rise is
+    // settled once instead, by a kernel of its own.
+    uint32_t* ordered = nullptr;
+    const uint32_t chunks = (r.rows + kRowsPerScan - 1) / kRowsPerScan;
+    const uint64_t block_rows = kThreads * kUnroll / (c.words <= 4 ? 4 : c.words <= 8 ? 8 : 16) /
+                                    r.kv_heads + 2;
+    if (c.row_stride == 0 && r.rows / kThreads * block_rows > 512 && s->rt) {
+        s->rt->activate();
+        cuda_check(cudaMalloc((void**)&ordered, chunks * 4ull), "cudaMalloc");
+        s->owned.push_back(ordered);
+        s->add("kv4_order", [=](cudaStream_t stream) {
+            return launch(stream, dim3(chunks), dim3(kRowsPerScan), 0, true, kv4_order_kernel, st,
+                          r.rows, ordered);
+        });
+    }
+    with_lanes(c.words, [&](auto lanes) {
+        constexpr int LPV = decltype(lanes)::value;
+        const dim3 grid(blocks_for((uint64_t)r.rows * r.kv_heads, LPV), 2);
+        auto go = [&](auto tag) {
+            using T = decltype(tag);
+            const T *k = (const T*)key.data, *v = (const T*)value.data;
+            s->add(label, [=](cudaStream_t stream) {
+                return launch(stream, grid, dim3(kThreads), 0, true, kv4_store_kernel<T, LPV>, k, v,
+                              c, r.rows, st, r.vec, (const uint32_t*)ordered, flags);
+            });
+        };
+        if (key.dtype == AB_F32) go(float());
+        else go(bf16());
+    });
+}
+
+}  // namespace ab
+
+using namespace ab;
+
+struct ab_kv4cache {
+    Runtime* rt;
+    uint32_t layers, batch, seq, kv_heads, head;
+    void* data[4];  // key codes, key scales, value codes, value scales
+    uint64_t vectors() const { return (uint64_t)layers * batch * kv_heads * seq; }
+    uint64_t bytes(int i) const { return vectors() * (i % 2 ? 4 : 4ull * kv4_words(head)); }
+};
+
+extern "C" {
+
+int ab_kernel_kv4_store(ab_scheme* s, ab_tensor key, ab_tensor value, const ab_kv4_layer* cache,
+                        ab_tensor step) {
+    return guard([&] {
+        if (!s || !cache) fail(AB_ERR_ARGUMENT, "null argument");
+        record_kv4_store(s, "kv4_store", key, value, *cache, step);
+    });
+}
+
+int ab_kernel_kv4_load(ab_scheme* s, const ab_kv4_layer* cache, ab_tensor step, ab_tensor key,
+                       ab_tensor value) {
+    return guard([&] {
+        if (!s || !cache) fail(AB_ERR_ARGUMENT, "null argument");
+        const Kv4Rows r = rows_of(key, value, 3, 4);
+        const uint32_t batch = key.rank == 4 ? key.dims[0] : 1;
+        const uint32_t n = key.dims[key.rank - 3];
+        const Kv4View c = kv4_operands(*cache, batch, r.kv_heads, r.head);
+        if (n > c.seq) invalid("parameter `key`: " + std::to_string(n) +
+                               " positions from a cache of " + std::to_string(c.seq));
+        expect_step(step, batch);
+        const Step* st = (const Step*)step.data;
+        uint32_t* flags = s->rt ? s->rt->flags : nullptr;
+        with_lanes(c.words, [&](auto lanes) {
+            constexpr int LPV = decltype(lanes)::value;
+            const dim3 grid(blocks_for((uint64_t)r.rows * r.kv_heads, LPV), 2);
+            auto go = [&](auto tag) {
+                using T = decltype(tag);
+                T *k = (T*)key.data, *v = (T*)value.data;
+                s->add("kv4_load", [=](cudaStream_t stream) {
+                    return launch(stream, grid, dim3(kThreads), 0, true, kv4_load_kernel<T, LPV>,
+                                  k, v, c, batch, n, st, r.vec, flags);
+                });
+            };
+            if (key.dtype == AB_F32) go(float());
+            else go(bf16());
+        });
+    });
+}
+
+int ab_kv4cache_create(ab_runtime* rt, uint32_t layers, uint32_t seq_len, uint32_t kv_heads,
+                       uint32_t head_size, uint32_t batch, ab_kv4cache** out) {
+    return guard([&] {
+        if (!rt || !out) fail(AB_ERR_ARGUMENT, "null argument");
+        if (!layers || !seq_len || !kv_heads || !head_size || !batch)
+            fail(AB_ERR_ARGUMENT, "Kv4Cache dims must be non-zero");
+        if (head_size > kKv4MaxHead)
+            fail(AB_ERR_ARGUMENT, "Kv4Cache head size must be at most 128");
+        auto* c = new ab_kv4cache{rt, layers, batch, seq_len, kv_heads, head_size, {}};
+        try {
+            rt->activate();
+            for (int i = 0; i < 4; i++) {
+                cuda_check(cudaMalloc(&c->data[i], c->bytes(i)), "cudaMalloc");
+                cuda_check(cudaMemset(c->data[i], 0, c->bytes(i)), "cudaMemset");
+            }
+        } catch (...) {
+            for (void* p : c->data)
+                if (p) cudaFree(p);
+            delete c;
+            throw;
+        }
+        *out = c;
+    });
+}
+
+int ab_kv4cache_layer(const ab_kv4cache* c, uint32_t layer, ab_kv4_layer* out) {
+    return guard([&] {
+        if (!c || !out) fail(AB_ERR_ARGUMENT, "null argument");
+        if (layer >= c->layers)
+            invalid("Kv4Cache::layer: layer " + std::to_string(layer) + " out of range (" +
+                    std::to_string(c->layers) + " layers)");
+        ab_tensor* t[4] = {&out->key_codes, &out->key_scales, &out->value_codes,
+                           &out->value_scales};
+        for (int i = 0; i < 4; i++) {
+            *t[i] = ab_tensor{};
+            t[i]->data = (char*)c->data[i] + layer * (c->bytes(i) / c->layers);
+            t[i]->dtype = AB_U32;
+            if (c->batch > 1) t[i]->dims[t[i]->rank++] = c->batch;
+            t[i]->dims[t[i]->rank++] = c->kv_heads;
+            t[i]->dims[t[i]->rank++] = c->seq;
+            if (i % 2 == 0) t[i]->dims[t[i]->rank++] = kv4_words(c->head);
+        }
+    });
+}
+
+int ab_kv4cache_zero(ab_kv4cache* c) {
+    return guard([&] {
+        if (!c) fail(AB_ERR_ARGUMENT, "null cache");
+        c->rt->activate();
+        for (int i = 0; i < 4; i++)
+            cuda_check(cudaMemsetAsync(c->data[i], 0, c->bytes(i), c->rt->stream), "zero cache");
+    });
+}
+
+int ab_kv4cache_destroy(ab_kv4cache* c) {
+    return guard([&] {
+        if (!c) return;
+        c->rt->activate();
+        cudaStreamSynchronize(c->rt->stream);
+        for (void* p : c->data) cudaFree(p);
+        delete c;
+    });
+}
+
+}  // extern "C"

@@ -1,0 +1,29 @@
+// The 4-bit key/value cache as the kernels see it (kv4.cu, kv4_attention.cu).
+#pragma once
+
+#include "internal.h"
+
+namespace ab {
+
+constexpr uint32_t kKv4MaxHead = 128;
+
+// 32-bit words of one vector's codes: eight elements a word, rows padded to 16 bytes.
+__host__ __device__ inline uint32_t kv4_words(uint32_t head) { return 4 * ((head + 31) / 32); }
+
+// One layer: codes [B,] kv_heads, seq, words and scales [B,] kv_heads, seq for keys (0) and
+// values (1). row_stride: vectors between the caches of consecutive rows (0: rows share one).
+struct Kv4View {
+    uint32_t* codes[2];
+    uint32_t* scales[2];
+    uint64_t row_stride;
+    uint32_t kv_heads, seq, head, words;
+};
+
+// Checks a layer for `rows` rows of kv_heads heads of size head.
+Kv4View kv4_operands(const ab_kv4_layer& c, uint32_t rows, uint32_t kv_heads, uint32_t head);
+
+// Quantises rows key/value [rows, kv_heads, head] into the cache at step[row].position.
+void record_kv4_store(ab_scheme* s, const char* label, ab_tensor key, ab_tensor value,
+                      const ab_kv4_layer& cache, ab_tensor step);
+
+}  // namespace ab

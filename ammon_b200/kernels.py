@@ -116,6 +116,48 @@ class AttentionDecodeKernel(_Kernel):
         return self._rec(scheme, q, key_cache, value_cache, out, step)
 
 
+class _Kv4Kernel(_Kernel):
+    def _rec4(self, scheme, cache, *args):
+        """args: tensors in the entry's order, with `cache` standing for its packed layer."""
+        from . import _check
+
+        layer = cache.c
+        _check(getattr(_abi.lib(), self.fn)(
+            scheme.handle, *[_abi.C.byref(layer) if a is cache else a.t for a in args]))
+        scheme.keep(*args)
+        return Dispatch()
+
+
+class Kv4StoreKernel(_Kv4Kernel):
+    """CacheStoreKernel for the 4-bit cache (Kv4Layer): quantises key and value rows
+    ([kv_heads, head] or [n, kv_heads, head]) at each row's step position."""
+
+    fn = "ab_kernel_kv4_store"
+
+    def record(self, scheme, label, key, value, cache, step):
+        return self._rec4(scheme, cache, key, value, cache, step)
+
+
+class Kv4LoadKernel(_Kv4Kernel):
+    """Reads positions from step.position on of a 4-bit cache back into key and value
+    [n, kv_heads, head] or [batch, n, kv_heads, head]."""
+
+    fn = "ab_kernel_kv4_load"
+
+    def record(self, scheme, label, cache, step, key, value):
+        return self._rec4(scheme, cache, cache, step, key, value)
+
+
+class Kv4AttentionKernel(_Kv4Kernel):
+    """AttentionDecodeKernel over a 4-bit cache (Kv4Layer): a cache per row, or one that all
+    rows share, each row attending over positions 0 .. its own."""
+
+    fn = "ab_kernel_kv4_attention"
+
+    def record(self, scheme, label, q, cache, out, step):
+        return self._rec4(scheme, cache, q, cache, out, step)
+
+
 class AttentionKernel(_Kernel):
     fn = "ab_kernel_attention"
 

@@ -199,6 +199,52 @@ int ab_kvcache_layer(const ab_kvcache* c, uint32_t layer, ab_tensor* key, ab_ten
 int ab_kvcache_zero(ab_kvcache* c);
 int ab_kvcache_destroy(ab_kvcache* c);
 
+/* ---- 4-bit key/value cache --------------------------------------------------------
+ * No counterpart in the reference, whose cache is f32 (src/modules.rs:38-64); beside KvCache,
+ * cache_store and attention_decode. A vector is what one kv head keeps for one position. It is
+ * held as 4-bit codes c_i and one word with two bf16 numbers, the step s (low half) and the
+ * offset m (high half), and stands for the values m + s c_i:
+ *     m = bf16(min x), s = bf16(max(max x - m, 0) / 15), c_i = (x_i - m) / s to the nearest
+ *     whole number (halves to even) within 0..15; all c_i are 0 where s is 0.
+ * A vector that holds an infinity or NaN, or whose range overflows, is NaN throughout.
+ * Codes are AB_U32 [kv_heads, seq, words] or [batch, kv_heads, seq, words], words =
+ * 4 * ceil(head / 32), 16-byte aligned: element i is bits 4 (i % 8) and up of word i / 8, the
+ * elements past head are 0. Scales are AB_U32 with the same dims but the last. head is 1..128.
+ * With a leading batch dim row b of a call uses cache b; without one all rows share the cache. */
+typedef struct {
+    ab_tensor key_codes, key_scales, value_codes, value_scales;
+} ab_kv4_layer;
+
+typedef struct ab_kv4cache ab_kv4cache;
+/* Zeroed caches of `layers` layers (zeroed vectors stand for zeros); layer() as
+ * ab_kvcache_layer: without the batch dim when batch == 1. */
+int ab_kv4cache_create(ab_runtime* rt, uint32_t layers, uint32_t seq_len, uint32_t kv_heads,
+                       uint32_t head_size, uint32_t batch, ab_kv4cache** out);
+int ab_kv4cache_layer(const ab_kv4cache* c, uint32_t layer, ab_kv4_layer* out);
+int ab_kv4cache_zero(ab_kv4cache* c);
+int ab_kv4cache_destroy(ab_kv4cache* c);
+
+/* Quantises key and value rows ([kv_heads, head] or [n, kv_heads, head], both f32 or both
+ * bf16) into the cache at step[row].position; nothing else of the cache is written. Of rows
+ * of one shared cache at the same position the last one is kept. A position >= seq writes
+ * nothing and raises AB_ERR_DEVICE at the next synchronising call. */
+int ab_kernel_kv4_store(ab_scheme* s, ab_tensor key, ab_tensor value, const ab_kv4_layer* cache,
+                        ab_tensor step);
+/* Reads back n <= seq positions from step[b].position on: key and value (both f32 or both
+ * bf16) are [n, kv_heads, head], or [batch, n, kv_heads, head] with one DecodeStep per batch
+ * row, the layouts of KvCache::layer. Positions >= seq give zeros and raise AB_ERR_DEVICE. */
+int ab_kernel_kv4_load(ab_scheme* s, const ab_kv4_layer* cache, ab_tensor step, ab_tensor key,
+                       ab_tensor value);
+/* Attention over positions [0, step[row].position] of the packed cache: q f32 [heads, head] or
+ * [batch, heads, head], out f32 or bf16 [batch, heads * head] (16-bit rounding only there);
+ * any whole number of query heads per kv head. With a batch dim each row has a cache of its
+ * own; without one all rows attend over the same cache, each up to its own position (the rows
+ * of a prompt). A row at a position >= seq gives zeros and raises AB_ERR_DEVICE. Positions
+ * past a row's own are never used, whatever they hold. Scratch is allocated here and owned by
+ * the scheme, which therefore needs a runtime. */
+int ab_kernel_kv4_attention(ab_scheme* s, ab_tensor q, const ab_kv4_layer* cache, ab_tensor out,
+                            ab_tensor step);
+
 /* CausalAttentionBlockWeights (src/modules.rs:13-19). */
 typedef struct {
     ab_tensor norm, query, key, value, output;

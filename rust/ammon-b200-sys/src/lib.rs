@@ -39,6 +39,16 @@ pub struct ab_decode_step {
     pub position: u32,
 }
 
+/// One layer of a 4-bit key/value cache (format: the header).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct ab_kv4_layer {
+    pub key_codes: ab_tensor,
+    pub key_scales: ab_tensor,
+    pub value_codes: ab_tensor,
+    pub value_scales: ab_tensor,
+}
+
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
 pub struct ab_attention_weights {
@@ -89,7 +99,7 @@ pub struct ab_autoregressive_model {
 macro_rules! opaque {
     ($($name:ident),*) => { $( #[repr(C)] pub struct $name { _private: [u8; 0] } )* };
 }
-opaque!(ab_runtime, ab_scheme, ab_kvcache, ab_attention_block, ab_swiglu_block, ab_llama,
+opaque!(ab_runtime, ab_scheme, ab_kvcache, ab_kv4cache, ab_attention_block, ab_swiglu_block, ab_llama,
         ab_comm, ab_bpe);
 
 extern "C" {
@@ -142,6 +152,13 @@ extern "C" {
     pub fn ab_kvcache_layer(c: *const ab_kvcache, layer: u32, key: *mut ab_tensor, value: *mut ab_tensor) -> c_int;
     pub fn ab_kvcache_zero(c: *mut ab_kvcache) -> c_int;
     pub fn ab_kvcache_destroy(c: *mut ab_kvcache) -> c_int;
+    pub fn ab_kv4cache_create(rt: *mut ab_runtime, layers: u32, seq_len: u32, kv_heads: u32, head_size: u32, batch: u32, out: *mut *mut ab_kv4cache) -> c_int;
+    pub fn ab_kv4cache_layer(c: *const ab_kv4cache, layer: u32, out: *mut ab_kv4_layer) -> c_int;
+    pub fn ab_kv4cache_zero(c: *mut ab_kv4cache) -> c_int;
+    pub fn ab_kv4cache_destroy(c: *mut ab_kv4cache) -> c_int;
+    pub fn ab_kernel_kv4_store(s: *mut ab_scheme, key: ab_tensor, value: ab_tensor, cache: *const ab_kv4_layer, step: ab_tensor) -> c_int;
+    pub fn ab_kernel_kv4_load(s: *mut ab_scheme, cache: *const ab_kv4_layer, step: ab_tensor, key: ab_tensor, value: ab_tensor) -> c_int;
+    pub fn ab_kernel_kv4_attention(s: *mut ab_scheme, q: ab_tensor, cache: *const ab_kv4_layer, out_: ab_tensor, step: ab_tensor) -> c_int;
     pub fn ab_attention_block_create(rt: *mut ab_runtime, hidden: u32, query_heads: u32, seq_len: u32, max_batch: u32, rope_theta: f32, out_: *mut *mut ab_attention_block) -> c_int;
     pub fn ab_attention_block_record(b: *mut ab_attention_block, s: *mut ab_scheme, x: ab_tensor, w: *const ab_attention_weights, key: ab_tensor, value: ab_tensor, step: ab_tensor) -> c_int;
     pub fn ab_attention_block_destroy(b: *mut ab_attention_block) -> c_int;
