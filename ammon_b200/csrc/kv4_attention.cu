@@ -17,15 +17,14 @@
 // lane's accumulators all belong to one head: its maximum, sum and rescaling need no exchange.
 //
 // Bound: the packed bytes. A warp's 32 positions (head 128) are 4352 bytes and about 400
-// instructions; a twelfth of them is mma. K, V and scales of the next 32 positions load into
-// registers straight from global memory while the present ones are computed.
+// instructions; a twelfth of them is mma. Each warp keeps the next 32 positions on their way into
+// shared memory while it computes on the present ones.
 //
-// Split: the tiles of all units (a row's or a slot block's positions of one kv head) form one
-// line that the teams of one wave of blocks share equally, so rows of unlike lengths and few
-// rows of great length fill the device alike. A team is a block's eight warps, 32 positions
-// each at a time, where units are few and long; a warp where they are many, so that short rows
-// do not pay for eight warps' start and joining. A unit that several teams meet is joined by
-// the last of them to finish, in line order: results do not depend on which that is.
+// Split: the tiles (a turn of all warps of a block) of all units (a row's or a slot block's
+// positions of one kv head) form one line that the blocks of one wave share equally, so rows of
+// unlike lengths and few rows of great length fill the device alike. A unit that several blocks
+// meet is joined by the last of them to finish, in line order: results do not depend on which
+// that is.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -35,6 +34,7 @@
 #include "common.cuh"
 #include "internal.h"
 #include "kv4.h"
+#include "tma.cuh"  // smem_u32
 
 namespace ab {
 
@@ -42,7 +42,11 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
-constexpr uint32_t kTurn = 32;   // positions of one warp's turn
+// Blocks of an SM. A third one (80 registers) measured 43 us instead of 37 at one row of 128k
+// positions, 70 instead of 73 at 256 rows of 512; one of 16 warps 37 and 101.
+constexpr int kResident = 2;
+constexpr uint32_t kTurn = 32;              // positions of one warp's turn
+constexpr uint32_t kTile = kWarps * kTurn;  // positions of one block's turn
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Kv4AttnParams {
@@ -53,8 +57,8 @@ struct Kv4AttnParams {
     uint32_t items;     // rows with a cache each, or blocks of query slots over one cache
     uint32_t per_item;  // kv heads x slot blocks of a row's group
     int shared;         // rows share one cache
-    int qvec, svec, ovec;  // 16-byte loads of q and of four scale words, four outputs at once
-    float* part;        // [2 teams][slots][32 W + 2] partial results
+    int qvec, ovec;     // 16-byte loads of q, four outputs at once
+    float* part;        // [2 grid][slots][32 W + 2] partial results
     uint32_t* tickets;  // [items * per_item], zero between launches
     const Step* step;
     uint32_t* flags;
@@ -75,6 +79,16 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// The same from zero.
+__device__ __forceinline__ void mma16816_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                              uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
 // 8 x 8 transpose of 16-bit elements held two a lane (row lane / 4, columns 2 (lane % 4) ..).
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t r;
@@ -90,63 +104,75 @@ __device__ __forceinline__ uint4 ld16(const void* p) {
                  : "l"(p));
     return r;
 }
-__device__ __forceinline__ uint2 ld8(const void* p) {
-    uint2 r;
-    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];"
-                 : "=r"(r.x), "=r"(r.y)
-                 : "l"(p));
-    return r;
-}
 __device__ __forceinline__ uint32_t ld4(const void* p) {
     uint32_t r;
     asm volatile("ld.global.u32 %0, [%1];" : "=r"(r) : "l"(p));
     return r;
 }
-__device__ __forceinline__ uint32_t ld2(const void* p) {
-    uint16_t r;
-    asm volatile("ld.global.u16 %0, [%1];" : "=h"(r) : "l"(p));
-    return r;
+// ---- a turn's rows in shared memory ---------------------------------------------------------
+// [32 rows of K codes][32 rows of V codes][K scales][V scales]. The 16-byte chunks of a row are
+// permuted by its number, so that eight consecutive rows of one chunk, which is what the lanes
+// read at a time, are in unlike banks (rows of 16 and 48 bytes are so by themselves).
+template <int W>
+struct Stage {
+    static constexpr uint32_t ROW = 16 * W;
+    static constexpr uint32_t V = kTurn * ROW, KS = 2 * V, VS = KS + 4 * kTurn;
+    static constexpr uint32_t BYTES = VS + 4 * kTurn;
+    __device__ __forceinline__ static uint32_t place(uint32_t row, uint32_t chunk) {
+        if constexpr (W == 4) chunk ^= row >> 1 & 3;
+        if constexpr (W == 2) chunk ^= row >> 2 & 1;
+        return row * ROW + chunk * 16;
+    }
+};
+constexpr uint32_t kStages = 2;
+
+// Asynchronous copies; those past the last row (size 0) write zeros and read nothing.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t size) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(size)
+                 : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, uint32_t size) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(size)
+                 : "memory");
+}
+__device__ __forceinline__ void copies_commit() {
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// W words: a lane's quarter of a K row.
+__device__ __forceinline__ uint32_t lds4(uint32_t at) {
+    uint32_t x;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(at) : "memory");
+    return x;
+}
+// A lane's quarter of a K row: W words.
 template <int W>
-__device__ __forceinline__ void load_k(const unsigned char* p, uint32_t (&w)[W]) {
+__device__ __forceinline__ void load_k(uint32_t at, uint32_t (&w)[W]) {
     if constexpr (W == 4) {
-        const uint4 r = ld16(p);
-        w[0] = r.x; w[1] = r.y; w[2] = r.z; w[3] = r.w;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                     : "r"(at)
+                     : "memory");
     } else if constexpr (W == 2) {
-        const uint2 r = ld8(p);
-        w[0] = r.x; w[1] = r.y;
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
+                     : "=r"(w[0]), "=r"(w[1])
+                     : "r"(at)
+                     : "memory");
     } else {
 #pragma unroll
-        for (int i = 0; i < W; i++) w[i] = ld4(p + 4 * i);
+        for (int i = 0; i < W; i++) w[i] = lds4(at + 4 * i);
     }
 }
-
-// A lane's eighth of a V row: W units of 16 bits (four dims each), two to a word where the
-// address allows (even W), else one.
-template <int W>
-constexpr int kVWords = W % 2 == 0 ? W / 2 : W;
-template <int W>
-__device__ __forceinline__ void load_v(const unsigned char* p, uint32_t (&w)[kVWords<W>]) {
-    if constexpr (W == 4) {
-        const uint2 r = ld8(p);
-        w[0] = r.x; w[1] = r.y;
-    } else if constexpr (W == 2) {
-        w[0] = ld4(p);
-    } else {
-#pragma unroll
-        for (int i = 0; i < W; i++) w[i] = ld2(p + 2 * i);
-    }
-}
-// Unit k of two rows side by side.
-template <int W>
-__device__ __forceinline__ uint32_t pair_units(const uint32_t (&a)[kVWords<W>],
-                                               const uint32_t (&b)[kVWords<W>], int k) {
-    if constexpr (W % 2 == 0)
-        return __byte_perm(a[k / 2], b[k / 2], k % 2 ? 0x7632 : 0x5410);
-    else
-        return __byte_perm(a[k], b[k], 0x5410);
+// One chunk (eight units of four codes) of all 32 V rows, transposed: y[b] holds unit r of the
+// rows 8 b + 2 c (low half) and 8 b + 2 c + 1. `at`: the chunk of row `lane`.
+__device__ __forceinline__ void load_v(uint32_t at, uint32_t (&y)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(y[0]), "=r"(y[1]), "=r"(y[2]), "=r"(y[3])
+                 : "r"(at)
+                 : "memory");
 }
 
 // One arrival at a ticket: what the block wrote before its last barrier is published with it,
@@ -175,38 +201,37 @@ __device__ __forceinline__ uint32_t item_length(const Kv4AttnParams& p, uint32_t
     }
     return n;
 }
-// Tiles of TILE positions; at least one, so that a row without positions is written too.
-template <uint32_t TILE>
+// Tiles of the line; at least one, so that a row without positions is written too.
 __device__ __forceinline__ uint32_t tiles_of(uint32_t length) {
-    return max(1u, (length + TILE - 1) / TILE);
+    return max(1u, (length + kTile - 1) / kTile);
 }
 
-// The line of `total` tiles over `teams` teams: the first `more` of them take one tile more.
+// The line of `total` tiles over `blocks` blocks: the first `more` of them take one tile more.
 struct Line {
-    uint32_t teams = 0, each = 0, more = 0;
+    uint32_t blocks = 0, each = 0, more = 0;
     __device__ __forceinline__ Line() {}
     __device__ __forceinline__ Line(uint32_t total, uint32_t most) {
-        teams = min(total, most);
-        each = total / teams;
-        more = total % teams;
+        blocks = min(total, most);
+        each = total / blocks;
+        more = total % blocks;
     }
-    __device__ __forceinline__ uint32_t begin(uint32_t team) const {
-        return team * each + min(team, more);
+    __device__ __forceinline__ uint32_t begin(uint32_t block) const {
+        return block * each + min(block, more);
     }
-    __device__ __forceinline__ uint32_t team_of(uint32_t tile) const {
+    __device__ __forceinline__ uint32_t block_of(uint32_t tile) const {
         const uint32_t cut = more * (each + 1);
         return tile < cut ? tile / (each + 1) : more + (tile - cut) / each;
     }
 };
 
-// What a team's first warp finds for all: its stretch, the unit at hand (tiles [at, until) of
-// the line) and the part of it that is the team's.
+// What a block's first warp finds for all: its stretch, the unit at hand (tiles [at, until) of
+// the line) and the part of it that is the block's.
 struct Span {
     uint32_t begin, end;
     uint32_t item, nth, kvh, sub, at, until, t_begin, t_end;
 };
 
-// A unit whose parts, those of teams first .. first + parts - 1, are to be joined.
+// A unit whose parts, those of blocks first .. first + parts - 1, are to be joined.
 struct Job {
     uint32_t item, kvh, sub, first, parts;
 };
@@ -260,137 +285,107 @@ struct Unit {
     }
 };
 
-template <int TEAM>
-__device__ __forceinline__ void team_sync() {
-    if constexpr (TEAM == 1) __syncwarp();
-    else __syncthreads();
-}
-
-// Joins the parts of teams first .. first + n - 1 in that order and writes the unit's rows.
-// [S][32 W] outputs are COLS groups of four; where these are fewer than the team's TT threads,
-// JG threads share one and take every JG-th part (what is left of the threads rests). A thread
-// joins its parts as an online softmax does, so that weights and values are read in one round,
-// AHEAD parts at a time. so, sm, sl: the team's shared arrays, free by now.
-template <int W, uint32_t S, int TEAM, typename OT>
+// Joins the parts of blocks first .. first + n - 1 in that order and writes the unit's rows.
+// The [S][32 W] outputs are COLS groups of four; JG threads share one and take every JG-th part
+// (what is left of the threads rests). A thread joins its parts as an online softmax does, so
+// that weights and values are read in one round, AHEAD parts at a time. so (a region of `stride`
+// floats a warp), sm, sl: the block's shared arrays, free by now.
+template <int W, uint32_t S, typename OT>
 __device__ __forceinline__ void join_parts(const Unit<W, S, OT>& unit, uint32_t first, uint32_t n,
-                                        uint32_t tt, float4* so, float (*sm)[S], float (*sl)[S]) {
-    constexpr uint32_t PART = S * (32 * W + 2), COLS = S * 8 * W, TT = TEAM * 32;
-    constexpr uint32_t JG = COLS < TT ? TT / COLS : 1;
-    constexpr uint32_t PER = COLS < TT ? 1 : COLS / TT;
-    constexpr uint32_t AHEAD = PER == 1 ? 8 : PER <= 4 ? 3 : 2;
-    static_assert(JG <= TEAM, "what a column's threads exchange fits where the warps' parts were");
-    const uint32_t col = tt % COLS, jg = COLS < TT ? tt / COLS : 0;
-    float4 x[PER];
-    float J[PER], L[PER];
-#pragma unroll
-    for (uint32_t k = 0; k < PER; k++) {
-        x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        J[k] = -INFINITY;
-        L[k] = 0.0f;
-    }
-    auto join = [&](uint32_t k, const float4& v, float mj, float lj) {
+                                        uint32_t tid, float* so, uint32_t stride, float (*sm)[S],
+                                           float (*sl)[S]) {
+    constexpr uint32_t PART = S * (32 * W + 2), COLS = S * 8 * W;
+    constexpr uint32_t JG = kThreads / COLS;
+    static_assert(JG >= 1 && JG <= kWarps, "exchanged values fit where the warps' parts were");
+    constexpr uint32_t AHEAD = 8;
+    const uint32_t col = tid % COLS, jg = tid / COLS;
+    const uint32_t s = col / (8 * W);
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float J = -INFINITY, L = 0.0f;
+    auto join = [&](const float4& v, float mj, float lj) {
         if (mj == -INFINITY) return;
-        const float to = fmaxf(J[k], mj), a = ex2(J[k] - to), b = ex2(mj - to);
-        x[k].x = fmaf(v.x, b, x[k].x * a);
-        x[k].y = fmaf(v.y, b, x[k].y * a);
-        x[k].z = fmaf(v.z, b, x[k].z * a);
-        x[k].w = fmaf(v.w, b, x[k].w * a);
-        L[k] = fmaf(lj, b, L[k] * a);
-        J[k] = to;
+        const float to = fmaxf(J, mj), a = ex2(J - to), b = ex2(mj - to);
+        x.x = fmaf(v.x, b, x.x * a);
+        x.y = fmaf(v.y, b, x.y * a);
+        x.z = fmaf(v.z, b, x.z * a);
+        x.w = fmaf(v.w, b, x.w * a);
+        L = fmaf(lj, b, L * a);
+        J = to;
     };
     for (uint32_t j0 = jg < JG ? jg : n; j0 < n; j0 += AHEAD * JG) {
-        float4 v[AHEAD][PER];
-        float mj[AHEAD][PER], lj[AHEAD][PER];
+        float4 v[AHEAD];
+        float mj[AHEAD], lj[AHEAD];
 #pragma unroll
         for (uint32_t u = 0; u < AHEAD; u++) {
             const uint32_t j = j0 + u * JG;
-            // the unit begins inside the first team's stretch and before the others'
+            // the unit begins inside the first block's stretch and before the others'
             const float* pj = unit.p.part + ((uint64_t)2 * (first + j) + (j == 0)) * PART;
-#pragma unroll
-            for (uint32_t k = 0; k < PER; k++) {
-                const uint32_t i = col + k * TT, s = i / (8 * W);
-                mj[u][k] = -INFINITY;
-                if (j < n) {
-                    mj[u][k] = __ldcg(pj + COLS * 4 + s);
-                    lj[u][k] = __ldcg(pj + COLS * 4 + S + s);
-                    v[u][k] = __ldcg(reinterpret_cast<const float4*>(pj) + i);
-                }
+            mj[u] = -INFINITY;
+            if (j < n) {
+                mj[u] = __ldcg(pj + COLS * 4 + s);
+                lj[u] = __ldcg(pj + COLS * 4 + S + s);
+                v[u] = __ldcg(reinterpret_cast<const float4*>(pj) + col);
             }
         }
 #pragma unroll
-        for (uint32_t u = 0; u < AHEAD; u++)
-#pragma unroll
-            for (uint32_t k = 0; k < PER; k++) join(k, v[u][k], mj[u][k], lj[u][k]);
+        for (uint32_t u = 0; u < AHEAD; u++) join(v[u], mj[u], lj[u]);
     }
     if constexpr (JG > 1) {
         if (jg < JG) {
-            so[jg * COLS + col] = x[0];
-            sm[jg][col / (8 * W)] = J[0];  // the same from every thread of a slot
-            sl[jg][col / (8 * W)] = L[0];
+            reinterpret_cast<float4*>(so + jg * stride)[col] = x;
+            sm[jg][s] = J;  // the same from every thread of a slot
+            sl[jg][s] = L;
         }
-        team_sync<TEAM>();
+        __syncthreads();
         if (jg == 0) {
 #pragma unroll
             for (uint32_t g = 1; g < JG; g++)
-                join(0, so[g * COLS + col], sm[g][col / (8 * W)], sl[g][col / (8 * W)]);
+                join(reinterpret_cast<const float4*>(so + g * stride)[col], sm[g][s], sl[g][s]);
         }
     }
-    if (jg == 0) {
-#pragma unroll
-        for (uint32_t k = 0; k < PER; k++) unit.write(col + k * TT, x[k], L[k]);
-    }
+    if (jg == 0) unit.write(col, x, L);
 }
 
-// W: words of codes in a quarter row (head up to 32 W). NT: four query slots each. TEAM: warps
-// that take a stretch of the line together (1 or 8).
-template <int W, int NT, int TEAM, typename OT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
+// W: words of codes in a quarter row (head up to 32 W). NT: four query slots each.
+template <int W, int NT, typename OT>
+__global__ void __launch_bounds__(kThreads, kResident)
     kv4_attention_kernel(const __grid_constant__ Kv4AttnParams p) {
     constexpr uint32_t S = 4 * NT;
     constexpr uint32_t HP = 32 * W;
     constexpr uint32_t ROW = 16 * W;  // bytes of a row of codes
     constexpr uint32_t PART = S * (HP + 2);
-    constexpr uint32_t TILE = TEAM * kTurn;
-    constexpr uint32_t TEAMS = kWarps / TEAM, TT = TEAM * 32;  // teams of a block, their threads
     constexpr uint32_t M0 = 0x000f000fu, M1 = 0x00f000f0u;
-    __shared__ float s_o[kWarps][S][HP];
+    using St = Stage<W>;
+    constexpr uint32_t RING = kStages * St::BYTES;  // a warp's turns; later its outputs [S][HP]
+    static_assert(S * HP * 4 <= RING && RING % 16 == 0, "outputs fit");
+    extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float s_m[kWarps][S], s_l[kWarps][S];
-    __shared__ float s_jm[TEAMS][S], s_jl[TEAMS][S];
-    __shared__ uint2 s_q[TEAM == 1 ? 1 : NT * W * 2][32];
-    __shared__ Slot s_slot[TEAMS][S];
-    __shared__ Span s_span[TEAMS];
-    __shared__ uint32_t s_scan[kWarps], s_item[TEAMS], s_at[TEAMS], s_jobs[TEAMS];
-    __shared__ Job s_job[TEAMS][2];
+    __shared__ float s_jm[S], s_jl[S];
+    __shared__ Slot s_slot[S];
+    __shared__ Span span;
+    __shared__ Job s_job[2];
+    __shared__ uint32_t s_scan[kWarps], s_item, s_at, s_jobs;
 
+    const uint32_t tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
     pdl_wait();
     pdl_trigger();
-    const uint32_t tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-    const uint32_t mate = warp % TEAM, crew = warp / TEAM, tt = tid % TT;
     const uint32_t r = lane / 4, c = lane % 4;
-    float (*so)[S][HP] = s_o + crew * TEAM;
-    float (*sm)[S] = s_m + crew * TEAM;
-    float (*sl)[S] = s_l + crew * TEAM;
-    Slot* slots = s_slot[crew];
-    Span& span = s_span[crew];
-    // the queries' operand columns; a lone warp keeps them where its outputs go later
-    uint2 (*qf)[32] = s_q;
-    if constexpr (TEAM == 1) {
-        static_assert(NT * W * 2 * 32 * sizeof(uint2) <= S * HP * sizeof(float), "q fits");
-        qf = reinterpret_cast<uint2 (*)[32]>(&so[0][0][0]);
-    }
+    unsigned char* ring = smem + warp * RING;
+    // the queries' operand columns
+    uint2 (*qf)[32] = reinterpret_cast<uint2 (*)[32]>(smem + kWarps * RING);
 
-    // ---- this team's stretch of the line --------------------------------------------------
+    // ---- this block's stretch of the line --------------------------------------------------
     if (blockIdx.x == 0) {
         for (uint32_t i = tid; i < p.rows; i += kThreads)
             if (p.step[i].position >= p.c.seq) atomicOr(p.flags, kFlagPositionRange);
     }
     uint32_t total = 0;  // tiles in all
     if (p.items == 1) {
-        if (mate == 0) total = tiles_of<TILE>(item_length<S>(p, 0)) * p.per_item;
+        if (warp == 0) total = tiles_of(item_length<S>(p, 0)) * p.per_item;
     } else {
         uint32_t sum = 0;
         for (uint32_t i = tid; i < p.items; i += kThreads)
-            sum += tiles_of<TILE>(item_length<S>(p, i));
+            sum += tiles_of(item_length<S>(p, i));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) s_scan[warp] = sum;
@@ -399,25 +394,25 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
         for (int w = 0; w < kWarps; w++) total += s_scan[w];
         total *= p.per_item;
     }
-    // Scalar work on the line is the team's first warp's; the others read what it found.
+    // Scalar work on the line is the first warp's; the others read what it found.
     Line line;
-    const uint32_t team = blockIdx.x * TEAMS + crew;
-    if (mate == 0) {
-        line = Line(total, gridDim.x * TEAMS);
+    if (warp == 0) {
+        line = Line(total, gridDim.x);
         if (lane == 0) {
-            span.begin = team < line.teams ? line.begin(team) : total;
-            span.end = team < line.teams ? line.begin(team + 1) : total;
+            const bool any = blockIdx.x < line.blocks;
+            span.begin = any ? line.begin(blockIdx.x) : total;
+            span.end = any ? line.begin(blockIdx.x + 1) : total;
         }
     }
-    if (TEAM > 1 || p.items > 1) __syncthreads();
-    else __syncwarp();
+    __syncthreads();
     const uint32_t begin = span.begin, end = span.end;
+    if (begin >= end) return;
     uint32_t item = 0, item_at = 0;  // tiles before `item`
     if (p.items > 1) {
         uint32_t base = 0;
         for (uint32_t i0 = 0; i0 < p.items; i0 += kThreads) {
             const uint32_t i = i0 + tid;
-            const uint32_t n = i < p.items ? tiles_of<TILE>(item_length<S>(p, i)) * p.per_item : 0;
+            const uint32_t n = i < p.items ? tiles_of(item_length<S>(p, i)) * p.per_item : 0;
             uint32_t upto = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -433,35 +428,30 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
                 if (w < warp) upto += s_scan[w];
                 base += s_scan[w];
             }
-#pragma unroll
-            for (uint32_t k = 0; k < TEAMS; k++) {
-                const uint32_t b = s_span[k].begin;
-                if (b < upto && b >= upto - n) {
-                    s_item[k] = i;
-                    s_at[k] = upto - n;
-                }
+            if (begin < upto && begin >= upto - n) {
+                s_item = i;
+                s_at = upto - n;
             }
-            if (base > s_span[TEAMS - 1].begin) break;
+            if (base > begin) break;
         }
         __syncthreads();
-        item = s_item[crew];
-        item_at = s_at[crew];
+        item = s_item;
+        item_at = s_at;
     }
 
-    // every later wait is a team's own
     uint32_t len = 0, n_tiles = 0, jobs = 0;
-    if (begin < end && mate == 0) {
+    if (warp == 0) {
         len = item_length<S>(p, item);
-        n_tiles = tiles_of<TILE>(len);
+        n_tiles = tiles_of(len);
     }
     for (uint32_t at = begin; at < end;) {
         // ---- the unit (item, kv head, slot block) at `at` ---------------------------------
-        if (mate == 0) {
+        if (warp == 0) {
             while (at - item_at >= n_tiles * p.per_item) {
                 item_at += n_tiles * p.per_item;
                 item++;
                 len = item_length<S>(p, item);
-                n_tiles = tiles_of<TILE>(len);
+                n_tiles = tiles_of(len);
             }
             const uint32_t nth = (at - item_at) / n_tiles;
             if (lane == 0) {
@@ -471,70 +461,53 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
                 span.kvh = nth - span.sub * p.c.kv_heads;
                 span.at = item_at + nth * n_tiles;
                 span.until = span.at + n_tiles;
-                span.t_begin = (at - span.at) * TILE;
-                span.t_end = min((min(end, span.until) - span.at) * TILE, len);
+                span.t_begin = (at - span.at) * kTile;
+                span.t_end = min((min(end, span.until) - span.at) * kTile, len);
             }
         }
-        team_sync<TEAM>();
+        __syncthreads();
         const Unit<W, S, OT> unit{p, span.item, span.kvh, span.sub};
         const uint32_t t_end = span.t_end;
         const uint64_t vec0 = (uint64_t)(p.shared ? 0 : unit.item) * p.c.row_stride +
                               (uint64_t)unit.kvh * p.c.seq;
 
-        // Position of index i of the 32, as an operand row: 4 r + 2 i + h of mma i, half h, for
-        // K rows, scales and scores; 4 (2 c + x) + 2 i + h for V. A lane's scales are one
-        // 16-byte word group.
-        const unsigned char* kbase = (const unsigned char*)p.c.codes[0] + vec0 * ROW + c * (4 * W);
-        const unsigned char* vbase = (const unsigned char*)p.c.codes[1] + vec0 * ROW + r * (2 * W);
-        const uint32_t* ksbase = p.c.scales[0] + vec0 + 4 * r;
-        const uint32_t* vsbase = p.c.scales[1] + vec0 + 4 * r;
-        uint32_t kw[2][2][W], vw[2][2][2][kVWords<W>], ks[4], vs[4];
-        auto load_scales = [&](const uint32_t* base, uint32_t t, uint32_t (&s)[4]) {
-            if (t + kTurn <= t_end && p.svec) {
-                const uint4 a = ld16(base + t);
-                s[0] = a.x; s[1] = a.y; s[2] = a.z; s[3] = a.w;
-            } else {
+        const unsigned char* ksrc =
+            (const unsigned char*)p.c.codes[0] + vec0 * ROW + lane * 16;
+        const unsigned char* vsrc =
+            (const unsigned char*)p.c.codes[1] + vec0 * ROW + lane * 16;
+        const uint32_t* kscale = p.c.scales[0] + vec0 + lane;
+        const uint32_t* vscale = p.c.scales[1] + vec0 + lane;
+        // The warp's turn at t into stage i, one group of copies (an empty one past the end).
+        // Chunk lane + 32 j is chunk (lane + 32 j) % W of row (lane + 32 j) / W.
+        auto fetch = [&](uint32_t t, uint32_t i) {
+            const uint32_t to = smem_u32(ring) + i * St::BYTES;
+            const unsigned char* k = ksrc + (uint64_t)t * ROW;
+            const unsigned char* v = vsrc + (uint64_t)t * ROW;
+            auto copy = [&](uint32_t n) {  // of n rows
 #pragma unroll
-                for (int i = 0; i < 4; i++) s[i] = t + 4 * r + i < t_end ? ld4(base + t + i) : 0;
-            }
+                for (uint32_t j = 0; j < W; j++) {
+                    const uint32_t row = (lane + 32 * j) / W;
+                    const uint32_t at = to + St::place(row, (lane + 32 * j) % W);
+                    const uint32_t size = row < n ? 16 : 0;
+                    copy16(at, k + (size ? j * 512 : 0), size);
+                    copy16(at + St::V, v + (size ? j * 512 : 0), size);
+                }
+                const uint32_t size = lane < n ? 4 : 0;
+                copy4(to + St::KS + 4 * lane, kscale + (size ? t : 0), size);
+                copy4(to + St::VS + 4 * lane, vscale + (size ? t : 0), size);
+            };
+            if (t + kTurn <= t_end) copy(kTurn);
+            else if (t < t_end) copy(t_end - t);
+            copies_commit();
         };
-        auto load_keys = [&](uint32_t t) {
-            if (t + kTurn <= t_end) {
-                const unsigned char* b = kbase + (uint64_t)(t + 4 * r) * ROW;
-#pragma unroll
-                for (int i = 0; i < 4; i++) load_k<W>(b + i * ROW, kw[i / 2][i % 2]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    load_k<W>(kbase + (uint64_t)min(t + 4 * r + i, t_end - 1) * ROW,
-                              kw[i / 2][i % 2]);
-            }
-            load_scales(ksbase, t, ks);
-        };
-        auto load_values = [&](uint32_t t) {
-            if (t + kTurn <= t_end) {
-                const unsigned char* b = vbase + (uint64_t)(t + 8 * c) * ROW;
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-                    load_v<W>(b + j * ROW, vw[j / 2 % 2][j % 2][j / 4]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-                    load_v<W>(vbase + (uint64_t)min(t + 8 * c + j, t_end - 1) * ROW,
-                              vw[j / 2 % 2][j % 2][j / 4]);
-            }
-            load_scales(vsbase, t, vs);
-        };
-        uint32_t t = span.t_begin + mate * kTurn;
-        if (t < t_end) {
-            load_keys(t);
-            load_values(t);
-        }
+        uint32_t t = span.t_begin + warp * kTurn;
+#pragma unroll 1
+        for (uint32_t i = 0; i < kStages; i++) fetch(t + i * kTile, i);
 
         // ---- queries, times log2(e) / sqrt(head), as operand columns -----------------------
         // Column 2 (s % 4) of slot s is the whole number next to q 2^e, the next one the rest;
         // e brings the head's largest |q| to [2^10, 2^11). A lane takes four dims.
-        for (uint32_t s = mate; s < S; s += TEAM) {
+        for (uint32_t s = warp; s < S; s += kWarps) {
             uint32_t row, head;
             const bool live = unit.slot(s, &row, &head);
             const uint32_t d0 = lane * 4, hd = p.c.head;
@@ -588,16 +561,16 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
                     const uint32_t pos = p.step[row].position;
                     limit = pos < p.c.seq ? (int32_t)pos : -1;
                 }
-                slots[s] = Slot{16777216.0f / up, sum, first * (-8.0f / 16777216.0f),
+                s_slot[s] = Slot{16777216.0f / up, sum, first * (-8.0f / 16777216.0f),
                                 rest * (-8.0f / 16777216.0f), limit};
             }
         }
-        team_sync<TEAM>();
+        __syncthreads();
         float qscale[NT], qsum[NT], qmid[NT][2];  // of slot c (+ 4 nt)
         int32_t limit[NT], lowest = 0x7fffffff;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            const Slot& q = slots[c + 4 * nt];
+            const Slot& q = s_slot[c + 4 * nt];
             qscale[nt] = q.scale;
             qsum[nt] = q.sum;
             qmid[nt][0] = q.first;
@@ -612,42 +585,51 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
         // Weights are w = 2^(score - M). M is the largest score + log2 step of V so far, less 9,
         // moved when a w x step reaches 2^11: as for the queries, its whole number is one operand
         // column, exact in the sums, and the rest the other.
-        float o[NT][2 * W][4], l[NT], pm[NT], M[NT], cap[NT];
+        float o[NT][2 * W][2], l[NT], pm[NT], M[NT], cap[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
             l[nt] = pm[nt] = M[nt] = 0.0f;
             cap[nt] = -1.0f;  // no position yet: any moves M
 #pragma unroll
-            for (int i = 0; i < 2 * W; i++) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.0f;
+            for (int i = 0; i < 2 * W; i++) o[nt][i][0] = o[nt][i][1] = 0.0f;
         }
-        for (; t < t_end; t += TILE) {
+        // Position 8 i + r of the 32, i = 0 .. 3, is lane r's: row r (even i) or 8 + r of the
+        // operand of K's mma i / 2; V's takes the rows in the same order.
+        const uint32_t k_at = W == 4   ? St::place(r, c)
+                              : W == 2 ? St::place(r, c / 2) + c % 2 * 8
+                                       : r * ROW + c * 4 * W;
+        uint32_t stage = 0;
+        for (; t < t_end; t += kTile) {
+            copies_wait<kStages - 1>();
+            __syncwarp();
+            const uint32_t st = smem_u32(ring) + stage * St::BYTES;
+            uint32_t ks[4], vs[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                ks[i] = lds4(st + St::KS + 4 * r + 32 * i);
+                vs[i] = lds4(st + St::VS + 4 * r + 32 * i);
+            }
             float acc[2][NT][4];
 #pragma unroll
-            for (int i = 0; i < 2; i++)
+            for (int i = 0; i < 2; i++) {
+                uint32_t kw[2][W];
+#pragma unroll
+                for (int h = 0; h < 2; h++) load_k<W>(st + k_at + (16 * i + 8 * h) * ROW, kw[h]);
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
                     acc[i][nt][0] = acc[i][nt][2] = qmid[nt][0];
                     acc[i][nt][1] = acc[i][nt][3] = qmid[nt][1];
                 }
 #pragma unroll
-            for (int w = 0; w < W; w++) {
-                uint2 b[NT][2];
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++) b[nt][h] = qf[(nt * W + w) * 2 + h][lane];
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const uint32_t x0 = kw[i][0][w], x1 = kw[i][1][w];
+                for (int w = 0; w < W; w++) {
+                    const uint32_t x0 = kw[0][w], x1 = kw[1][w];
                     const uint32_t y0 = x0 >> 8, y1 = x1 >> 8;
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-                        mma16816(acc[i][nt], x0 & M0, x1 & M0, x0 & M1, x1 & M1, b[nt][0].x,
-                                 b[nt][0].y);
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-                        mma16816(acc[i][nt], y0 & M0, y1 & M0, y0 & M1, y1 & M1, b[nt][1].x,
-                                 b[nt][1].y);
+                    for (int nt = 0; nt < NT; nt++) {
+                        const uint2 b0 = qf[(nt * W + w) * 2][lane], b1 = qf[(nt * W + w) * 2 + 1][lane];
+                        mma16816(acc[i][nt], x0 & M0, x1 & M0, x0 & M1, x1 & M1, b0.x, b0.y);
+                        mma16816(acc[i][nt], y0 & M0, y1 & M0, y0 & M1, y1 & M1, b1.x, b1.y);
+                    }
                 }
             }
             // score - M = s (q . (c - 8)) + (m + 8 s) sum q - M, taken off M first: the exact
@@ -664,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
                         float x = fmaf(acc[i / 2][nt][2 * (i % 2)], sq, -M[nt]);
                         x = fmaf(acc[i / 2][nt][2 * (i % 2) + 1], sq, x);
                         x = fmaf(fmaf(8.0f, step, bf16hi(ks[i])), qsum[nt], x);
-                        const bool out = masked.value && (int32_t)(t + 4 * r + i) > limit[nt];
+                        const bool out = masked.value && (int32_t)(t + 8 * i + r) > limit[nt];
                         sc[nt][i] = out ? -INFINITY : x;
                         w[nt][i] = ex2(sc[nt][i]);
                         ws[nt][i] = out ? 0.0f : w[nt][i] * bf16lo(vs[i]);
@@ -696,8 +678,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
                             pm[nt] *= a;
 #pragma unroll
                             for (int i = 0; i < 2 * W; i++) {
-                                o[nt][i][0] *= a; o[nt][i][1] *= a;
-                                o[nt][i][2] *= a; o[nt][i][3] *= a;
+                                o[nt][i][0] *= a;
+                                o[nt][i][1] *= a;
                             }
                         }
                         cap[nt] = 2048.0f;
@@ -705,14 +687,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
                 }
                 weigh(std::true_type());
             }
-            if (t + TILE < t_end) load_keys(t + TILE);
             uint32_t pb[NT][4];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     l[nt] += w[nt][i];
-                    if (!masked || (int32_t)(t + 4 * r + i) <= limit[nt])
+                    if (!masked || (int32_t)(t + 8 * i + r) <= limit[nt])
                         pm[nt] = fmaf(w[nt][i], bf16hi(vs[i]), pm[nt]);
                     // the nearest whole number, by way of 1.5 2^23
                     const float first = (ws[nt][i] + 12582912.0f) - 12582912.0f;
@@ -720,40 +701,39 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
                     pb[nt][i] = transpose8(*reinterpret_cast<const uint32_t*>(&two));
                 }
             }
-            // Sums of 32 positions start from zero and are added to the running ones here: the
-            // unit's own addition cuts off, and over a long chain of positive terms that shows
-            // (1.4e-5 at 128k positions).
+            // Sums of 32 positions start from zero and are added to the running ones, the rest's
+            // with the whole numbers', here: the unit's own addition cuts off, and over a long
+            // chain of positive terms that shows (1.4e-5 at 128k positions).
 #pragma unroll
-            for (int k = 0; k < W; k++) {
-                uint32_t y[2][2], z[2][2];
+            for (uint32_t k = 0; k < W; k++) {
+                uint32_t y[4];
+                load_v(st + St::V + St::place(lane, k), y);
 #pragma unroll
-                for (int i = 0; i < 2; i++)
+                for (int b = 0; b < 2; b++) {
+                    if (b) {
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        y[i][h] = pair_units<W>(vw[i][h][0], vw[i][h][1], k);
-                        z[i][h] = y[i][h] >> 8;
+                        for (int i = 0; i < 4; i++) y[i] >>= 8;
                     }
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    float a[2][4] = {};
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        mma16816(a[0], y[i][0] & M0, y[i][0] & M1, y[i][1] & M0, y[i][1] & M1,
-                                 pb[nt][2 * i], pb[nt][2 * i + 1]);
-                        mma16816(a[1], z[i][0] & M0, z[i][0] & M1, z[i][1] & M0, z[i][1] & M1,
-                                 pb[nt][2 * i], pb[nt][2 * i + 1]);
+                    for (int nt = 0; nt < NT; nt++) {
+                        float a[4];
+                        mma16816_zero(a, y[0] & M0, y[0] & M1, y[1] & M0, y[1] & M1, pb[nt][0],
+                                      pb[nt][1]);
+                        mma16816(a, y[2] & M0, y[2] & M1, y[3] & M0, y[3] & M1, pb[nt][2],
+                                 pb[nt][3]);
+                        o[nt][2 * k + b][0] += a[0] + a[1];
+                        o[nt][2 * k + b][1] += a[2] + a[3];
                     }
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-#pragma unroll
-                        for (int x = 0; x < 4; x++) o[nt][2 * k + h][x] += a[h][x];
                 }
             }
-            if (t + TILE < t_end) load_values(t + TILE);
+            __syncwarp();  // every lane is done with the stage
+            fetch(t + kStages * kTile, stage);
+            stage = (stage + 1) % kStages;
         }
 
         // ---- the warps' parts joined -----------------------------------------------------------
-        if constexpr (TEAM == 1) __syncwarp();  // all lanes are done with the queries
+        __syncwarp();
+        float* mo = reinterpret_cast<float*>(ring);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -763,112 +743,104 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
             }
             if (r == 0) {
                 // no positions: no part (a sum that is NaN is one)
-                sm[mate][c + 4 * nt] = l[nt] == 0.0f ? -INFINITY : M[nt];
-                sl[mate][c + 4 * nt] = l[nt];
+                s_m[warp][c + 4 * nt] = l[nt] == 0.0f ? -INFINITY : M[nt];
+                s_l[warp][c + 4 * nt] = l[nt];
             }
 #pragma unroll
             for (int i = 0; i < 2 * W; i++) {
-                const uint32_t d = (r * W + i / 2) * 4 + 2 * (i % 2);
-                *reinterpret_cast<float2*>(&so[mate][c + 4 * nt][d]) =
-                    make_float2(fmaf(o[nt][i][0] + o[nt][i][1], 16777216.0f, pm[nt]),
-                                fmaf(o[nt][i][2] + o[nt][i][3], 1048576.0f, pm[nt]));
+                const uint32_t d = (8 * (i / 2) + r) * 4 + 2 * (i % 2);
+                *reinterpret_cast<float2*>(mo + (c + 4 * nt) * HP + d) =
+                    make_float2(fmaf(o[nt][i][0], 16777216.0f, pm[nt]),
+                                fmaf(o[nt][i][1], 1048576.0f, pm[nt]));
             }
         }
-        team_sync<TEAM>();
-        float *jm = s_jm[crew], *jl = s_jl[crew];
-        if (tt < S) {
-            float J = -INFINITY, L = 0.0f;
-#pragma unroll
-            for (int w = 0; w < TEAM; w++) J = fmaxf(J, sm[w][tt]);
-#pragma unroll
-            for (int w = 0; w < TEAM; w++) {
-                const float a = sm[w][tt] == -INFINITY ? 0.0f : ex2(sm[w][tt] - J);
-                L = fmaf(sl[w][tt], a, L);
-                sm[w][tt] = a;
+        __syncthreads();
+        static_assert(kWarps <= 32, "a lane per warp");
+        for (uint32_t s = warp; s < S; s += kWarps) {
+            const float m = lane < kWarps ? s_m[lane][s] : -INFINITY;
+            const float J = warp_max(m), a = m == -INFINITY ? 0.0f : ex2(m - J);
+            const float L = warp_sum(lane < kWarps ? s_l[lane][s] * a : 0.0f);
+            if (lane < kWarps) s_m[lane][s] = a;
+            if (lane == 0) {
+                s_jm[s] = J;
+                s_jl[s] = L;
             }
-            jm[tt] = J;
-            jl[tt] = L;
         }
-        team_sync<TEAM>();
+        __syncthreads();
         const bool whole = begin <= span.at && span.until <= end;
-        // a unit that began in an earlier stretch is this team's first part, else its last
-        float* mine = p.part + (uint64_t)(2 * team + (begin <= span.at)) * PART;
-        for (uint32_t i = tt; i < S * HP / 4; i += TT) {
+        // a unit that began in an earlier stretch is this block's first part, else its last
+        float* mine = p.part + (uint64_t)(2 * blockIdx.x + (begin <= span.at)) * PART;
+        const float* so = reinterpret_cast<const float*>(smem);
+        for (uint32_t i = tid; i < S * HP / 4; i += kThreads) {
             const uint32_t s = i * 4 / HP, d = i * 4 % HP;
             float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-            for (int w = 0; w < TEAM; w++) {
-                const float4 v = *reinterpret_cast<const float4*>(&so[w][s][d]);
-                const float a = sm[w][s];
+            for (int w = 0; w < kWarps; w++) {
+                const float4 v = *reinterpret_cast<const float4*>(so + w * (RING / 4) + s * HP + d);
+                const float a = s_m[w][s];
                 x.x = fmaf(v.x, a, x.x);
                 x.y = fmaf(v.y, a, x.y);
                 x.z = fmaf(v.z, a, x.z);
                 x.w = fmaf(v.w, a, x.w);
             }
-            if (whole) unit.write(i, x, jl[s]);
+            if (whole) unit.write(i, x, s_jl[s]);
             else __stcg(reinterpret_cast<float4*>(mine) + i, x);
         }
         if (!whole) {
-            if (tt < S) {
-                __stcg(mine + S * HP + tt, jm[tt]);
-                __stcg(mine + S * HP + S + tt, jl[tt]);
+            if (tid < S) {
+                __stcg(mine + S * HP + tid, s_jm[tid]);
+                __stcg(mine + S * HP + S + tid, s_jl[tid]);
             }
-            team_sync<TEAM>();  // the team's part is written; its first thread publishes it
-            if (tt == 0) {
-                // teams first .. last meet this unit; the last to arrive joins their parts, after
+            __syncthreads();  // the block's part is written; its first thread publishes it
+            if (tid == 0) {
+                // blocks first .. last meet this unit; the last to arrive joins their parts, after
                 // its stretch: up to two units, those at the stretch's ends
-                const uint32_t first = line.team_of(span.at);
-                const uint32_t parts = line.team_of(span.until - 1) - first + 1;
+                const uint32_t first = line.block_of(span.at);
+                const uint32_t parts = line.block_of(span.until - 1) - first + 1;
                 uint32_t* ticket = p.tickets + (uint64_t)unit.item * p.per_item + span.nth;
                 if (arrive(ticket) == parts - 1) {
                     *ticket = 0;
-                    s_job[crew][jobs++] = Job{unit.item, unit.kvh, unit.sub, first, parts};
+                    s_job[jobs++] = Job{unit.item, unit.kvh, unit.sub, first, parts};
                 }
             }
         }
         at = min(end, span.until);
-        team_sync<TEAM>();  // the next unit reuses the shared arrays
+        __syncthreads();  // the next unit reuses the shared arrays
     }
-    if (tt == 0) s_jobs[crew] = jobs;
-    team_sync<TEAM>();
-    for (uint32_t k = 0; k < s_jobs[crew]; k++) {
-        const Job& job = s_job[crew][k];
-        join_parts<W, S, TEAM>(Unit<W, S, OT>{p, job.item, job.kvh, job.sub}, job.first, job.parts,
-                               tt, reinterpret_cast<float4*>(so), sm, sl);
-        team_sync<TEAM>();
+    if (tid == 0) s_jobs = jobs;
+    __syncthreads();
+    for (uint32_t k = 0; k < s_jobs; k++) {
+        const Job& job = s_job[k];
+        join_parts<W, S>(Unit<W, S, OT>{p, job.item, job.kvh, job.sub}, job.first, job.parts,
+                         tid, reinterpret_cast<float*>(smem), RING / 4, s_m, s_l);
+        __syncthreads();
     }
 }
 
-template <int W, int NT, int TEAM, typename OT>
-void record_one(ab_scheme* s, Kv4AttnParams p, uint32_t grid) {
+template <int W, int NT, typename OT>
+void record_one(ab_scheme* s, Kv4AttnParams p) {
     constexpr uint32_t S = 4 * NT, PART = S * (32 * W + 2);
-    auto* kernel = kv4_attention_kernel<W, NT, TEAM, OT>;
-    const uint64_t units = (uint64_t)p.items * p.per_item;
-    const uint64_t tiles = units * ((p.c.seq + TEAM * kTurn - 1) / (TEAM * kTurn));
-    if (tiles >> 31) invalid("kv4_attention: too much work for one call");
-    grid = (uint32_t)std::min<uint64_t>(grid, (tiles * TEAM + kWarps - 1) / kWarps);
-    const uint64_t part_bytes = (uint64_t)grid * (kWarps / TEAM) * 2 * PART * 4;
-    unsigned char* scratch = nullptr;
+    constexpr size_t smem = kWarps * kStages * Stage<W>::BYTES +
+                            NT * W * 2 * 32 * sizeof(uint2);
+    auto* kernel = kv4_attention_kernel<W, NT, OT>;
     s->rt->activate();
+    cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+               "kv4_attention shared memory");
+    const uint64_t units = (uint64_t)p.items * p.per_item;
+    const uint64_t tiles = units * ((p.c.seq + kTile - 1) / kTile);
+    if (tiles >> 31) invalid("kv4_attention: too much work for one call");
+    const uint32_t grid = (uint32_t)std::min<uint64_t>(
+        (uint64_t)s->rt->sm_count * kResident, tiles);
+    const uint64_t part_bytes = (uint64_t)grid * 2 * PART * 4;
+    unsigned char* scratch = nullptr;
     cuda_check(cudaMalloc((void**)&scratch, part_bytes + units * 4), "cudaMalloc");
     s->owned.push_back(scratch);
     cuda_check(cudaMemset(scratch + part_bytes, 0, units * 4), "clear tickets");
     p.part = (float*)scratch;
     p.tickets = (uint32_t*)(scratch + part_bytes);
     s->add("kv4_attention", [=](cudaStream_t stream) {
-        return launch(stream, dim3(grid), dim3(kThreads), 0, true, kernel, p);
+        return launch(stream, dim3(grid), dim3(kThreads), smem, true, kernel, p);
     });
-}
-
-template <int W, int NT>
-void record_slots(ab_scheme* s, const Kv4AttnParams& p, int32_t out_dtype) {
-    // one wave; a warp to a team where each unit then meets about eight teams or fewer
-    const uint32_t grid = (uint32_t)s->rt->sm_count * (NT == 1 ? 2 : 1);
-    const bool solo = (uint64_t)p.items * p.per_item >= grid;
-    if (out_dtype == AB_F32)
-        solo ? record_one<W, NT, 1, float>(s, p, grid) : record_one<W, NT, 8, float>(s, p, grid);
-    else
-        solo ? record_one<W, NT, 1, bf16>(s, p, grid) : record_one<W, NT, 8, bf16>(s, p, grid);
 }
 
 template <int W>
@@ -880,8 +852,9 @@ void record_width(ab_scheme* s, Kv4AttnParams p, int32_t out_dtype) {
     const uint32_t blocks = (uint32_t)((slots + S - 1) / S);
     p.items = p.shared ? blocks : p.rows;
     p.per_item = p.c.kv_heads * (p.shared ? 1 : blocks);
-    if (S == 4) record_slots<W, 1>(s, p, out_dtype);
-    else record_slots<W, 2>(s, p, out_dtype);
+    const bool f32 = out_dtype == AB_F32;
+    if (S == 4) f32 ? record_one<W, 1, float>(s, p) : record_one<W, 1, bf16>(s, p);
+    else f32 ? record_one<W, 2, float>(s, p) : record_one<W, 2, bf16>(s, p);
 }
 
 }  // namespace
@@ -927,8 +900,6 @@ extern "C" int ab_kernel_kv4_attention(ab_scheme* s, ab_tensor q, const ab_kv4_l
         p.heads = heads;
         p.group = heads / kv;
         p.qvec = head % 4 == 0 && (uintptr_t)q.data % 16 == 0;
-        p.svec = p.c.seq % 4 == 0 &&
-                 ((uintptr_t)p.c.scales[0] | (uintptr_t)p.c.scales[1]) % 16 == 0;
         p.ovec = head % 4 == 0 && (uintptr_t)out.data % (4 * dtype_size(out.dtype)) == 0;
         p.step = (const Step*)step.data;
         p.flags = s->rt->flags;
