@@ -94,17 +94,41 @@ __device__ __forceinline__ void load8(const T* p, uint32_t left, bool vec, float
     }
 }
 
-// The code of x: the whole number nearest to (x - m) / s in real arithmetic, halves to even,
-// within 0..15. u = fl(fl(x - m) * fl(1 / s)) is within 3 * 2^-24 * 16 < 3e-6 of the quotient
-// wherever |u| <= 16, so it decides every case but those within 1e-5 of a half; these, and
-// steps whose reciprocal is not a normal number, take the quotient in 64 bits.
-__device__ __forceinline__ uint32_t code_of(float x, float m, float s, float inv) {
-    const float u = fminf(fmaxf((x - m) * inv, -1.0f), 16.0f);
-    const float k = rintf(u);
-    if (fabsf(u - k) < 0.49999f && inv < 1e37f) return (uint32_t)fminf(fmaxf(k, 0.0f), 15.0f);
-    const double q = ((double)x - (double)m) / (double)s;
-    return (uint32_t)fmin(fmax(rint(q), 0.0), 15.0);
+// ---- codes -------------------------------------------------------------------------------
+// The code of x is the whole number nearest to (x - m) / s in real arithmetic, halves to even,
+// within 0..15. u = fl(fl(x - m) * fl(1 / (15 s))), cut to 0..1, times 15 is within 5 * 2^-24 * 15
+// < 5e-6 of the quotient, which decides every case but those that close to a half: about one
+// word in ten thousand goes to exact_word.
+constexpr float kNearHalf = 0.499995f;
+constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number
+
+// The same for a whole word, decided exactly in 32 bits. With d = fl(x - m) and its error e,
+// x - m - h s has the sign of fma(-h, s, d) + e: h s (h a half, s of 8 bits) enters exactly, and
+// where it is near d the difference is exact. Elements are read again: the caller's are in
+// registers, and a loop keeps this path short.
+template <typename T>
+__device__ __noinline__ uint32_t exact_word(const T* p, uint32_t left, float m, float s) {
+    const float up = s < 0x1p-100f ? 0x1p64f : 1.0f;  // a reciprocal that is a normal number
+    const float inv = 1.0f / (s * up);
+    uint32_t word = 0;
+    for (uint32_t i = 0; i < min(left, 8u); i++) {
+        const float x = to_f32(p[i]), d = x - m;
+        const float back = d - x, e = (x - (d - back)) + (-m - back);
+        float k = rintf(fminf(fmaxf(d * up * inv, 0.0f), 15.0f));
+        const bool odd = ((int)k & 1) != 0;
+        const float over = fmaf(-(k + 0.5f), s, d) + e, under = fmaf(0.5f - k, s, d) + e;
+        if (over > 0.0f || (over == 0.0f && odd)) k += 1.0f;
+        else if (under < 0.0f || (under == 0.0f && odd)) k -= 1.0f;
+        word |= (uint32_t)fminf(fmaxf(k, 0.0f), 15.0f) << (4 * i);
+    }
+    return word;
 }
+
+// Vectors go to lane groups in order, kv heads fastest: a group's next one is GROUPS further,
+// `lines` lines and `heads` heads on.
+struct Walk {
+    uint32_t total, lines, heads;
+};
 
 constexpr uint32_t kRowsPerScan = 1024;
 
@@ -126,7 +150,7 @@ __global__ void __launch_bounds__(kRowsPerScan)
 template <typename T, int LPV>
 __global__ void __launch_bounds__(kThreads)
     kv4_store_kernel(const T* key, const T* value, const Kv4View c,
-                     uint32_t rows, const Step* step, int vec,
+                     const Walk walk, uint32_t rows, const Step* step, int vec,
                      const uint32_t* ordered, uint32_t* flags) {
     constexpr uint32_t GROUPS = kThreads / LPV;
     constexpr uint32_t VECS = GROUPS * kUnroll;
@@ -134,21 +158,30 @@ __global__ void __launch_bounds__(kThreads)
     pdl_wait();
     const uint32_t which = blockIdx.y;
     const T* src = which ? value : key;
-    const uint64_t total = (uint64_t)rows * c.kv_heads;
-    const uint64_t v0 = (uint64_t)blockIdx.x * VECS;
+    uint32_t* codes = which ? c.codes[1] : c.codes[0];
+    uint32_t* scales = which ? c.scales[1] : c.scales[0];
+    const uint32_t v0 = blockIdx.x * VECS;
     const uint32_t sub = threadIdx.x % LPV, grp = threadIdx.x / LPV;
     const uint32_t e0 = sub * 8;
     const uint32_t left = e0 < c.head ? c.head - e0 : 0;
     float x[kUnroll][8];
     uint32_t row[kUnroll], kvh[kUnroll], pos[kUnroll];
+    row[0] = (v0 + grp) / c.kv_heads;
+    kvh[0] = (v0 + grp) - row[0] * c.kv_heads;
 #pragma unroll
     for (int u = 0; u < kUnroll; u++) {
-        const uint64_t v = v0 + u * GROUPS + grp;
-        const bool live = v < total;
-        row[u] = live ? (uint32_t)(v / c.kv_heads) : 0;
-        kvh[u] = live ? (uint32_t)(v % c.kv_heads) : 0;
+        if (u) {
+            row[u] = row[u - 1] + walk.lines;
+            kvh[u] = kvh[u - 1] + walk.heads;
+            if (kvh[u] >= c.kv_heads) {
+                kvh[u] -= c.kv_heads;
+                row[u]++;
+            }
+        }
+        const uint32_t v = v0 + u * GROUPS + grp;
+        const bool live = v < walk.total;
         pos[u] = live ? step[row[u]].position : 0xffffffffu;
-        load8(src + (live ? v * c.head + e0 : 0), live ? left : 0, vec, x[u]);
+        load8(src + (live ? (uint64_t)v * c.head + e0 : 0), live ? left : 0, vec, x[u]);
         if (live && pos[u] >= c.seq && sub == 0) atomicOr(flags, kFlagPositionRange);
     }
     // rows of one cache at the same position: the last one is written. Rising positions (a
@@ -161,8 +194,8 @@ __global__ void __launch_bounds__(kThreads)
         scan = !__syncthreads_and(ok);
     }
     if (scan) {
-        const uint32_t r0 = (uint32_t)(v0 / c.kv_heads);
-        const uint32_t r1 = (uint32_t)min((uint64_t)rows, (v0 + VECS - 1) / c.kv_heads + 1);
+        const uint32_t r0 = v0 / c.kv_heads;
+        const uint32_t r1 = min(rows, (v0 + VECS - 1) / c.kv_heads + 1);
         for (uint32_t r = threadIdx.x; r < VECS; r += kThreads) lost[r] = 0;
         __syncthreads();
         for (uint32_t q = r0 + 1 + threadIdx.x; q < rows; q += kThreads) {
@@ -198,18 +231,34 @@ __global__ void __launch_bounds__(kThreads)
         const bf16 sb = __float2bfloat16_rn(__fdiv_rn(fmaxf(__fsub_rn(hi, m), 0.0f), 15.0f));
         const float s = __bfloat162float(sb);
         const bool bad = !(fin == 0.0f) || !isfinite(m) || !isfinite(s);
+        const bool write = pos[u] < c.seq;
         uint32_t word = 0;
         if (!bad && s > 0.0f) {
-            const float inv = 1.0f / s;
+            const float inv = 1.0f / (15.0f * s);
+            float near = s < 0x1p-100f ? 1.0f : 0.0f, half[2];
 #pragma unroll
-            for (uint32_t i = 0; i < 8; i++)
-                if (i < left) word |= code_of(x[u][i], m, s, inv) << (4 * i);
+            for (int h = 0; h < 2; h++) {
+                float k[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float f = __saturatef((x[u][4 * h + i] - m) * inv);
+                    k[i] = fmaf(f, 15.0f, kMagic) - kMagic;
+                    near = fmaxf(near, fabsf(fmaf(f, 15.0f, -k[i])));
+                }
+                // four codes as one whole number below 2^16
+                half[h] = fmaf(fmaf(fmaf(k[3], 16.0f, k[2]), 16.0f, k[1]), 16.0f, k[0]);
+            }
+            word = (__float_as_uint(half[0] + kMagic) & 0xffffu) |
+                   __float_as_uint(half[1] + kMagic) << 16;
+            if (near > kNearHalf && write)
+                word = exact_word(src + ((uint64_t)(v0 + u * GROUPS + grp) * c.head + e0), left, m, s);
+            if (left < 8) word &= left ? 0xffffffffu >> (32 - 4 * left) : 0u;
         }
-        if (pos[u] >= c.seq) continue;
+        if (!write) continue;
         const uint64_t at = (uint64_t)row[u] * c.row_stride + (uint64_t)kvh[u] * c.seq + pos[u];
-        if (sub < c.words) c.codes[which][at * c.words + sub] = word;
+        if (sub < c.words) codes[at * c.words + sub] = word;
         if (sub == 0)
-            c.scales[which][at] = bad ? 0x7fff7fffu
+            scales[at] = bad ? 0x7fff7fffu
                                       : (uint32_t)__bfloat16_as_ushort(sb) |
                                             ((uint32_t)__bfloat16_as_ushort(mb) << 16);
     }
@@ -220,7 +269,7 @@ __global__ void __launch_bounds__(kThreads)
 // end give zeros and raise the position flag.
 template <typename T, int LPV>
 __global__ void __launch_bounds__(kThreads)
-    kv4_load_kernel(T* key, T* value, const Kv4View c, uint32_t batch, uint32_t n,
+    kv4_load_kernel(T* key, T* value, const Kv4View c, const Walk walk, uint32_t n,
                     const Step* step, int vec, uint32_t* flags) {
     constexpr uint32_t GROUPS = kThreads / LPV;
     constexpr uint32_t VECS = GROUPS * kUnroll;
@@ -228,37 +277,47 @@ __global__ void __launch_bounds__(kThreads)
     pdl_trigger();
     const uint32_t which = blockIdx.y;
     T* dst = which ? value : key;
-    const uint64_t total = (uint64_t)batch * n * c.kv_heads;
+    const uint32_t* codes = which ? c.codes[1] : c.codes[0];
+    const uint32_t* scales = which ? c.scales[1] : c.scales[0];
     const uint32_t sub = threadIdx.x % LPV, grp = threadIdx.x / LPV;
     const uint32_t e0 = sub * 8;
+    const uint32_t v0 = blockIdx.x * VECS + grp;
+    uint32_t line = v0 / c.kv_heads, kvh = v0 - line * c.kv_heads;
+    uint32_t b = line / n, i = line - b * n;
     uint32_t word[kUnroll], sc[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; u++) {
-        const uint64_t v = (uint64_t)blockIdx.x * VECS + u * GROUPS + grp;
         word[u] = sc[u] = 0;
-        if (v < total) {
-            const uint64_t line = v / c.kv_heads;
-            const uint32_t kvh = (uint32_t)(v % c.kv_heads);
-            const uint32_t b = (uint32_t)(line / n);
-            const uint64_t pos = (uint64_t)step[b].position + line % n;
+        if (v0 + u * GROUPS < walk.total) {
+            const uint64_t pos = (uint64_t)step[b].position + i;
             if (pos < c.seq) {
                 const uint64_t at = (uint64_t)b * c.row_stride + (uint64_t)kvh * c.seq + pos;
-                if (sub < c.words) word[u] = __ldcg(c.codes[which] + at * c.words + sub);
-                sc[u] = __ldcg(c.scales[which] + at);
+                if (sub < c.words) word[u] = __ldcg(codes + at * c.words + sub);
+                sc[u] = __ldcg(scales + at);
             } else if (sub == 0) {
                 atomicOr(flags, kFlagPositionRange);
             }
         }
+        kvh += walk.heads;
+        i += walk.lines;
+        if (kvh >= c.kv_heads) {
+            kvh -= c.kv_heads;
+            i++;
+        }
+        if (i >= n) {
+            b += i / n;
+            i %= n;
+        }
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; u++) {
-        const uint64_t v = (uint64_t)blockIdx.x * VECS + u * GROUPS + grp;
-        if (v >= total || e0 >= c.head) continue;
+        const uint32_t v = v0 + u * GROUPS;
+        if (v >= walk.total || e0 >= c.head) continue;
         const float s = bf16lo(sc[u]), m = bf16hi(sc[u]);
         float x[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) x[i] = fmaf((float)((word[u] >> (4 * i)) & 15u), s, m);
-        T* p = dst + v * c.head + e0;
+        T* p = dst + (uint64_t)v * c.head + e0;
         if (vec) {
             if constexpr (sizeof(T) == 2) {
                 uint4 r;
@@ -313,11 +372,13 @@ void with_lanes(uint32_t words, F&& f) {
     else f(std::integral_constant<int, 16>());
 }
 
-unsigned blocks_for(uint64_t vectors, int lanes) {
-    const uint64_t per = (uint64_t)kThreads / lanes * kUnroll;
-    const uint64_t n = (vectors + per - 1) / per;
-    if (n > 0x7fffffffu) invalid("kv4: too many vectors for one call");
-    return (unsigned)n;
+// The walk of rows x kv_heads vectors by groups of `lanes`, and its blocks.
+Walk walk_of(const Kv4Rows& r, int lanes, unsigned* blocks) {
+    const uint64_t total = (uint64_t)r.rows * r.kv_heads;
+    if (total >> 31) invalid("parameter `key`: too many vectors for one call");
+    const uint32_t groups = kThreads / lanes;
+    *blocks = (unsigned)((total + groups * kUnroll - 1) / (groups * kUnroll));
+    return Walk{(uint32_t)total, groups / r.kv_heads, groups % r.kv_heads};
 }
 
 }  // namespace
@@ -347,13 +408,14 @@ void record_kv4_store(ab_scheme* s, const char* label, ab_tensor key, ab_tensor 
     }
     with_lanes(c.words, [&](auto lanes) {
         constexpr int LPV = decltype(lanes)::value;
-        const dim3 grid(blocks_for((uint64_t)r.rows * r.kv_heads, LPV), 2);
+        unsigned blocks = 0;
+        const Walk walk = walk_of(r, LPV, &blocks);
         auto go = [&](auto tag) {
             using T = decltype(tag);
             const T *k = (const T*)key.data, *v = (const T*)value.data;
             s->add(label, [=](cudaStream_t stream) {
-                return launch(stream, grid, dim3(kThreads), 0, true, kv4_store_kernel<T, LPV>, k, v,
-                              c, r.rows, st, r.vec, (const uint32_t*)ordered, flags);
+                return launch(stream, dim3(blocks, 2), dim3(kThreads), 0, true,
+                              kv4_store_kernel<T, LPV>, k, v, c, walk, r.rows, st, r.vec, (const uint32_t*)ordered, flags);
             });
         };
         if (key.dtype == AB_F32) go(float());
@@ -398,13 +460,14 @@ int ab_kernel_kv4_load(ab_scheme* s, const ab_kv4_layer* cache, ab_tensor step, 
         uint32_t* flags = s->rt ? s->rt->flags : nullptr;
         with_lanes(c.words, [&](auto lanes) {
             constexpr int LPV = decltype(lanes)::value;
-            const dim3 grid(blocks_for((uint64_t)r.rows * r.kv_heads, LPV), 2);
+            unsigned blocks = 0;
+            const Walk walk = walk_of(r, LPV, &blocks);
             auto go = [&](auto tag) {
                 using T = decltype(tag);
                 T *k = (T*)key.data, *v = (T*)value.data;
                 s->add("kv4_load", [=](cudaStream_t stream) {
-                    return launch(stream, grid, dim3(kThreads), 0, true, kv4_load_kernel<T, LPV>,
-                                  k, v, c, batch, n, st, r.vec, flags);
+                    return launch(stream, dim3(blocks, 2), dim3(kThreads), 0, true,
+                                  kv4_load_kernel<T, LPV>, k, v, c, walk, n, st, r.vec, flags);
                 });
             };
             if (key.dtype == AB_F32) go(float());
