@@ -89,18 +89,34 @@ __device__ __forceinline__ void load8(const T* p, uint32_t left, bool vec, float
             v[6] = __uint_as_float(b.z); v[7] = __uint_as_float(b.w);
         }
     } else {
+        // past the row's end: its first element here again, which changes no extreme
 #pragma unroll
-        for (uint32_t i = 0; i < 8; i++) v[i] = i < left ? to_f32(p[i]) : 0.0f;
+        for (uint32_t i = 0; i < 8; i++) v[i] = left ? to_f32(p[i < left ? i : 0]) : 0.0f;
     }
 }
 
 // ---- codes -------------------------------------------------------------------------------
 // The code of x is the whole number nearest to (x - m) / s in real arithmetic, halves to even,
-// within 0..15. u = fl(fl(x - m) * fl(1 / (15 s))), cut to 0..1, times 15 is within 5 * 2^-24 * 15
-// < 5e-6 of the quotient, which decides every case but those that close to a half: about one
-// word in ten thousand goes to exact_word.
+// within 0..15. f = fl(fl(x - m) * fl(1 / (15 s))), cut to 0..1, times 15 is within 5 * 2^-24 * 15
+// < 5e-6 of the quotient, which decides every case but those that close to a half.
+//   f32 rows: these are about one word in ten thousand; exact_word decides them.
+//   bf16 rows: quotients of 8-bit numbers, they are halves or well apart from them, and halves
+//   are common. With k = rne(15 f), d - k s is exact, and is +-s / 2 for a half: the even
+//   neighbour is then 2 rne(7.5 f). Only where x is lost in x - m (2^16 below it) is a half left
+//   to exact_word.
 constexpr float kNearHalf = 0.499995f;
 constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number
+
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 
 // The same for a whole word, decided exactly in 32 bits. With d = fl(x - m) and its error e,
 // x - m - h s has the sign of fma(-h, s, d) + e: h s (h a half, s of 8 bits) enters exactly, and
@@ -211,46 +227,56 @@ __global__ void __launch_bounds__(kThreads)
     pdl_trigger();
 #pragma unroll
     for (int u = 0; u < kUnroll; u++) {
-        float lo = INFINITY, hi = -INFINITY, fin = 0.0f;
+        float lo = x[u][0], hi = x[u][0];  // NaN once a value is
 #pragma unroll
-        for (uint32_t i = 0; i < 8; i++) {
-            if (i < left) {
-                lo = fminf(lo, x[u][i]);
-                hi = fmaxf(hi, x[u][i]);
-                fin = fmaf(x[u][i], 0.0f, fin);  // NaN once a value is not finite
-            }
+        for (int i = 1; i < 8; i++) {
+            lo = min_nan(lo, x[u][i]);
+            hi = max_nan(hi, x[u][i]);
+        }
+        if (left == 0) {
+            lo = INFINITY;
+            hi = -INFINITY;
         }
 #pragma unroll
         for (int o = LPV / 2; o > 0; o >>= 1) {
-            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-            fin += __shfl_xor_sync(0xffffffffu, fin, o);
+            lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         }
         const bf16 mb = __float2bfloat16_rn(lo);
         const float m = __bfloat162float(mb);
         const bf16 sb = __float2bfloat16_rn(__fdiv_rn(fmaxf(__fsub_rn(hi, m), 0.0f), 15.0f));
         const float s = __bfloat162float(sb);
-        const bool bad = !(fin == 0.0f) || !isfinite(m) || !isfinite(s);
+        // a value of the row, its range or its offset is not finite
+        const bool bad = !(isfinite(lo) && isfinite(hi) && isfinite(m) && isfinite(s));
         const bool write = pos[u] < c.seq;
         uint32_t word = 0;
         if (!bad && s > 0.0f) {
             const float inv = 1.0f / (15.0f * s);
-            float near = s < 0x1p-100f ? 1.0f : 0.0f, half[2];
+            bool exactly = s < 0x1p-100f;
+            float near = 0.0f, half[2];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 float k[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float f = __saturatef((x[u][4 * h + i] - m) * inv);
+                    const float v = x[u][4 * h + i], d = v - m;
+                    const float f = __saturatef(d * inv);
                     k[i] = fmaf(f, 15.0f, kMagic) - kMagic;
-                    near = fmaxf(near, fabsf(fmaf(f, 15.0f, -k[i])));
+                    if constexpr (sizeof(T) == 4) {
+                        near = fmaxf(near, fabsf(fmaf(f, 15.0f, -k[i])));
+                    } else {
+                        const float even = fmaf(f, 7.5f, kMagic) - kMagic;
+                        const bool tie = fabsf(fmaf(-k[i], s, d)) == 0.5f * s;
+                        exactly |= tie && d + m != v;
+                        k[i] = tie ? even + even : k[i];
+                    }
                 }
                 // four codes as one whole number below 2^16
                 half[h] = fmaf(fmaf(fmaf(k[3], 16.0f, k[2]), 16.0f, k[1]), 16.0f, k[0]);
             }
             word = (__float_as_uint(half[0] + kMagic) & 0xffffu) |
                    __float_as_uint(half[1] + kMagic) << 16;
-            if (near > kNearHalf && write)
+            if ((exactly || near > kNearHalf) && write)
                 word = exact_word(src + ((uint64_t)(v0 + u * GROUPS + grp) * c.head + e0), left, m, s);
             if (left < 8) word &= left ? 0xffffffffu >> (32 - 4 * left) : 0u;
         }
