@@ -1235,7 +1235,7 @@ extern "C" int ab_kernel_attention_decode(ab_scheme* s, ab_tensor q, ab_tensor k
         void* counters = nullptr;
         cuda_check(cudaMalloc(&part, std::max<uint64_t>(floats, 1) * 4), "cudaMalloc");
         if (cudaMalloc(&counters, tickets * 4) != cudaSuccess ||
-            cudaMemset(counters, 0, tickets * 4) != cudaSuccess) {
+            clear_device(s->rt, counters, tickets * 4) != cudaSuccess) {
             cudaGetLastError();
             cudaFree(part);
             if (counters) cudaFree(counters);

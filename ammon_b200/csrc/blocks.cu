@@ -74,7 +74,7 @@ void* device_alloc(Runtime* rt, size_t bytes) {
     void* p = nullptr;
     rt->activate();
     cuda_check(cudaMalloc(&p, std::max<size_t>(bytes, 16)), "cudaMalloc");
-    cuda_check(cudaMemset(p, 0, std::max<size_t>(bytes, 16)), "cudaMemset");
+    cuda_check(clear_device(rt, p, std::max<size_t>(bytes, 16)), "clear");
     return p;
 }
 

@@ -825,11 +825,11 @@ void alloc_tc_scratch(Runtime* rt, GemmScratch* g, uint32_t max_batch, uint32_t 
         // bf16 activation rows, or the fp32 hi and lo halves of the 3xTF32 path
         t.xn_bytes = (uint64_t)max_batch * max_k * 8;
         cuda_check(cudaMalloc(&t.xn, t.xn_bytes), "cudaMalloc");
-        cuda_check(cudaMemset(t.xn, 0, t.xn_bytes), "cudaMemset");
+        cuda_check(clear_device(rt, t.xn, t.xn_bytes), "clear");
         gemm_tc_scratch(max_tiles, max_batch, rt->sm_count, &t.ws_floats, &t.tickets_n);
         cuda_check(cudaMalloc(&t.ws, t.ws_floats * 4), "cudaMalloc");
         cuda_check(cudaMalloc(&t.tickets, (size_t)t.tickets_n * 4), "cudaMalloc");
-        cuda_check(cudaMemset(t.tickets, 0, (size_t)t.tickets_n * 4), "cudaMemset");
+        cuda_check(clear_device(rt, t.tickets, (size_t)t.tickets_n * 4), "clear");
     } catch (...) {
         free_tc_scratch(&t);
         throw;

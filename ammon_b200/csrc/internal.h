@@ -103,6 +103,14 @@ struct Runtime {
     void set_wait_limit_ms(uint64_t ms);  // writes the limit into the flag block
 };
 
+// Zeroes device memory before anything recorded or copied on the runtime's stream can reach it.
+// (A plain cudaMemset runs on the default stream, which the runtime's does not wait for: it could
+// clear memory that a copy or a kernel on the runtime's stream had already filled.)
+inline cudaError_t clear_device(const Runtime* rt, void* p, size_t bytes) {
+    const cudaError_t e = cudaMemsetAsync(p, 0, bytes, rt->stream);
+    return e == cudaSuccess ? cudaStreamSynchronize(rt->stream) : e;
+}
+
 enum DeviceFlag : uint32_t {
     kFlagTokenRange = 1u,
     kFlagPositionRange = 2u,

@@ -515,7 +515,7 @@ int ab_kv4cache_create(ab_runtime* rt, uint32_t layers, uint32_t seq_len, uint32
             rt->activate();
             for (int i = 0; i < 4; i++) {
                 cuda_check(cudaMalloc(&c->data[i], c->bytes(i)), "cudaMalloc");
-                cuda_check(cudaMemset(c->data[i], 0, c->bytes(i)), "cudaMemset");
+                cuda_check(clear_device(rt, c->data[i], c->bytes(i)), "clear");
             }
         } catch (...) {
             for (void* p : c->data)

@@ -835,7 +835,7 @@ void record_one(ab_scheme* s, Kv4AttnParams p) {
     unsigned char* scratch = nullptr;
     cuda_check(cudaMalloc((void**)&scratch, part_bytes + units * 4), "cudaMalloc");
     s->owned.push_back(scratch);
-    cuda_check(cudaMemset(scratch + part_bytes, 0, units * 4), "clear tickets");
+    cuda_check(clear_device(s->rt, scratch + part_bytes, units * 4), "clear tickets");
     p.part = (float*)scratch;
     p.tickets = (uint32_t*)(scratch + part_bytes);
     s->add("kv4_attention", [=](cudaStream_t stream) {

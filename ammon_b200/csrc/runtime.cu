@@ -358,10 +358,10 @@ int ab_tensor_zeros(ab_runtime* rt, int32_t dtype, int32_t rank, const uint32_t*
         if (bytes == 0) fail(AB_ERR_ARGUMENT, "zero-sized tensor");
         rt->activate();
         cuda_check(cudaMalloc(&t.data, bytes), "cudaMalloc");
-        cudaError_t e = cudaMemset(t.data, 0, bytes);
+        cudaError_t e = clear_device(rt, t.data, bytes);
         if (e != cudaSuccess) {
             cudaFree(t.data);
-            cuda_check(e, "cudaMemset");
+            cuda_check(e, "clear tensor");
         }
         *out = t;
     });

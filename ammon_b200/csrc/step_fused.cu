@@ -1194,7 +1194,7 @@ FusedStep* fused_step_create(Runtime* rt, const FusedStepModel& m) {
         b_layers + b_q + b_o + b_h + b_x2 + b_part + b_ml + b_tk + b_cand + b_bar + b_trace;
     try {
         cuda_check(cudaMalloc(&f->scratch, total), "fused step scratch");
-        cuda_check(cudaMemset(f->scratch, 0, total), "fused step scratch");
+        cuda_check(clear_device(rt, f->scratch, total), "fused step scratch");
         char* c = (char*)f->scratch;
         PsLayer* layers = (PsLayer*)c;
         c += b_layers;
