@@ -106,7 +106,7 @@ void Runtime::check_flags() {
     uint32_t f = 0;
     cuda_check(cudaMemcpy(&f, flags, 4, cudaMemcpyDeviceToHost), "read device flags");
     if (f) {
-        cuda_check(cudaMemset(flags, 0, 4), "clear device flags");
+        cuda_check(clear_device(this, flags, 4), "clear device flags");
         fail(AB_ERR_DEVICE, device_flag_message(f));
     }
 }
