@@ -61,7 +61,7 @@ Kv4View kv4_operands(const ab_kv4_layer& c, uint32_t rows, uint32_t kv_heads, ui
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;  // vectors a lane group has in flight
+constexpr int kLoadUnroll = 4;  // vectors a lane group of the load has in flight
 
 // 16 bytes that are read once. Not the non-coherent path: this grid may have started while the
 // kernel that writes them still ran.
@@ -73,40 +73,7 @@ __device__ __forceinline__ uint4 ld_once(const void* p) {
     return r;
 }
 
-// Eight elements of a row from element e on (`left` of them exist; vec: 16-byte loads).
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, uint32_t left, bool vec, float* v) {
-    if (vec && left >= 8) {
-        if constexpr (sizeof(T) == 2) {
-            const uint4 r = ld_once(p);
-            v[0] = bf16lo(r.x); v[1] = bf16hi(r.x); v[2] = bf16lo(r.y); v[3] = bf16hi(r.y);
-            v[4] = bf16lo(r.z); v[5] = bf16hi(r.z); v[6] = bf16lo(r.w); v[7] = bf16hi(r.w);
-        } else {
-            const uint4 a = ld_once(p), b = ld_once(p + 4);
-            v[0] = __uint_as_float(a.x); v[1] = __uint_as_float(a.y);
-            v[2] = __uint_as_float(a.z); v[3] = __uint_as_float(a.w);
-            v[4] = __uint_as_float(b.x); v[5] = __uint_as_float(b.y);
-            v[6] = __uint_as_float(b.z); v[7] = __uint_as_float(b.w);
-        }
-    } else {
-        // past the row's end: its first element here again, which changes no extreme
-#pragma unroll
-        for (uint32_t i = 0; i < 8; i++) v[i] = left ? to_f32(p[i < left ? i : 0]) : 0.0f;
-    }
-}
-
-// ---- codes -------------------------------------------------------------------------------
-// The code of x is the whole number nearest to (x - m) / s in real arithmetic, halves to even,
-// within 0..15. f = fl(fl(x - m) * fl(1 / (15 s))), cut to 0..1, times 15 is within 5 * 2^-24 * 15
-// < 5e-6 of the quotient, which decides every case but those that close to a half.
-//   f32 rows: these are about one word in ten thousand; exact_word decides them.
-//   bf16 rows: quotients of 8-bit numbers, they are halves or well apart from them, and halves
-//   are common. With k = rne(15 f), d - k s is exact, and is +-s / 2 for a half: the even
-//   neighbour is then 2 rne(7.5 f). Only where x is lost in x - m (2^16 below it) is a half left
-//   to exact_word.
-constexpr float kNearHalf = 0.499995f;
-constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number
-
+// Smaller and larger, NaN if either is.
 __device__ __forceinline__ float min_nan(float a, float b) {
     float r;
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -117,6 +84,116 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
+__device__ __forceinline__ uint32_t min_nan2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t max_nan2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+// Eight elements of a row as they were read: bf16 in pairs, f32.
+template <typename T>
+struct Eight;
+template <>
+struct Eight<float> {
+    float v[8];
+    __device__ __forceinline__ float at(int i) const { return v[i]; }
+    __device__ __forceinline__ void load(const float* p) {
+        const uint4 a = ld_once(p), b = ld_once(p + 4);
+        v[0] = __uint_as_float(a.x); v[1] = __uint_as_float(a.y);
+        v[2] = __uint_as_float(a.z); v[3] = __uint_as_float(a.w);
+        v[4] = __uint_as_float(b.x); v[5] = __uint_as_float(b.y);
+        v[6] = __uint_as_float(b.z); v[7] = __uint_as_float(b.w);
+    }
+    __device__ __forceinline__ void set(int i, float x) { v[i] = x; }
+};
+// Smallest and largest of a vector, two Eights (`any`: the first has elements; the second holds
+// some of them) in each of LPV lanes; NaN if one is.
+template <int LPV>
+__device__ __forceinline__ void extremes(const Eight<float> (&e)[2], bool any, float* lo,
+                                         float* hi) {
+    float l = e[0].v[0], h = l;
+#pragma unroll
+    for (int i = 1; i < 16; i++) {
+        l = min_nan(l, e[i / 8].v[i % 8]);
+        h = max_nan(h, e[i / 8].v[i % 8]);
+    }
+    if (!any) {
+        l = INFINITY;
+        h = -INFINITY;
+    }
+#pragma unroll
+    for (int o = LPV / 2; o > 0; o >>= 1) {
+        l = min_nan(l, __shfl_xor_sync(0xffffffffu, l, o));
+        h = max_nan(h, __shfl_xor_sync(0xffffffffu, h, o));
+    }
+    *lo = l;
+    *hi = h;
+}
+template <>
+struct Eight<bf16> {
+    uint32_t w[4];
+    __device__ __forceinline__ float at(int i) const {
+        return i % 2 ? bf16hi(w[i / 2]) : bf16lo(w[i / 2]);
+    }
+    __device__ __forceinline__ void load(const bf16* p) {
+        const uint4 a = ld_once(p);
+        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+    }
+    __device__ __forceinline__ void set(int i, bf16 x) {
+        const uint32_t b = __bfloat16_as_ushort(x);
+        w[i / 2] = i % 2 ? w[i / 2] | b << 16 : b;
+    }
+};
+// In pairs; then the smallest and minus the largest as one pair.
+template <int LPV>
+__device__ __forceinline__ void extremes(const Eight<bf16> (&e)[2], bool any, float* lo,
+                                         float* hi) {
+    uint32_t l = e[0].w[0], h = l;
+#pragma unroll
+    for (int i = 1; i < 8; i++) {
+        l = min_nan2(l, e[i / 4].w[i % 4]);
+        h = max_nan2(h, e[i / 4].w[i % 4]);
+    }
+    h ^= 0x80008000u;
+    uint32_t x = min_nan2(__byte_perm(l, h, 0x5410), __byte_perm(l, h, 0x7632));
+    if (!any) x = 0x7f807f80u;  // infinities
+#pragma unroll
+    for (int o = LPV / 2; o > 0; o >>= 1) x = min_nan2(x, __shfl_xor_sync(0xffffffffu, x, o));
+    *lo = bf16lo(x);
+    *hi = -bf16hi(x);
+}
+// `left` elements of the row exist from p on (vec: 16-byte loads, whole eights). Past the row's
+// end its first element here stands again, which changes no extreme.
+template <typename T>
+__device__ __forceinline__ void load16(const T* p, uint32_t left, bool vec, Eight<T> (&e)[2]) {
+    if (vec) {
+        if (left) e[0].load(p);
+        if (left > 8) e[1].load(p + 8);
+        else e[1] = e[0];
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 16; i++)
+            e[i / 8].set(i % 8, left ? p[i < left ? i : 0] : from_f32<T>(0.0f));
+    }
+}
+
+// ---- codes -------------------------------------------------------------------------------
+// The code of x is the whole number nearest to (x - m) / s in real arithmetic, halves to even,
+// within 0..15. f = fl(fl(x - m) * fl(1 / (15 s))), cut to 0..1, times 15 is within 5 * 2^-24 * 15
+// < 5e-6 of the quotient, which decides every case but those that close to a half.
+//   f32 rows: these are about one word in ten thousand; exact_word decides them.
+//   bf16 rows: quotients of 8-bit numbers, they are halves or well apart from them, and halves
+//   are common. With k = rne(15 f) and d = x - m, d - k s is exact, and is +-s / 2 for a half: the
+//   even neighbour is then 2 rne(7.5 f). d itself is inexact only where x is 2^16 below m, or m
+//   below x: rows where the quotient next to that, -m / s or x / s, may be a half, go to
+//   exact_word whole (m / s a half, one row in a hundred; 0 < |m| < s / 2^11).
+constexpr float kNearHalf = 0.499995f;
+constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number
 
 // The same for a whole word, decided exactly in 32 bits. With d = fl(x - m) and its error e,
 // x - m - h s has the sign of fma(-h, s, d) + e: h s (h a half, s of 8 bits) enters exactly, and
@@ -159,17 +236,21 @@ __global__ void __launch_bounds__(kRowsPerScan)
     if (threadIdx.x == 0) ordered[blockIdx.x] = all;
 }
 
-// LPV lanes hold one vector, eight elements (one code word) each; a block takes kUnroll *
-// kThreads / LPV consecutive vectors of one of the two tensors (blockIdx.y), kv heads fastest,
-// so its loads are one contiguous run of the source. All of a lane's loads are issued before
-// the first is used.
+// LPV lanes hold one vector, sixteen elements (two code words) each; a block takes U * kThreads /
+// LPV consecutive vectors of one of the two tensors (blockIdx.y), kv heads fastest, so its loads
+// are one contiguous run of the source. All of a lane's loads are issued before the first is
+// used. Bound by instructions (a row of 128: its offset, step and checks once for 16 elements,
+// 12 instructions an element); with eight elements a lane it was half as slow again.
+template <typename T>
+constexpr int kStoreUnroll = sizeof(T) == 2 ? 4 : 2;
 template <typename T, int LPV>
 __global__ void __launch_bounds__(kThreads)
     kv4_store_kernel(const T* key, const T* value, const Kv4View c,
                      const Walk walk, uint32_t rows, const Step* step, int vec,
                      const uint32_t* ordered, uint32_t* flags) {
+    constexpr int U = kStoreUnroll<T>;
     constexpr uint32_t GROUPS = kThreads / LPV;
-    constexpr uint32_t VECS = GROUPS * kUnroll;
+    constexpr uint32_t VECS = GROUPS * U;
     __shared__ uint32_t lost[VECS];  // per row of this block: a later row has its position
     pdl_wait();
     const uint32_t which = blockIdx.y;
@@ -178,14 +259,14 @@ __global__ void __launch_bounds__(kThreads)
     uint32_t* scales = which ? c.scales[1] : c.scales[0];
     const uint32_t v0 = blockIdx.x * VECS;
     const uint32_t sub = threadIdx.x % LPV, grp = threadIdx.x / LPV;
-    const uint32_t e0 = sub * 8;
+    const uint32_t e0 = sub * 16;
     const uint32_t left = e0 < c.head ? c.head - e0 : 0;
-    float x[kUnroll][8];
-    uint32_t row[kUnroll], kvh[kUnroll], pos[kUnroll];
+    Eight<T> x[U][2];
+    uint32_t row[U], kvh[U], pos[U];
     row[0] = (v0 + grp) / c.kv_heads;
     kvh[0] = (v0 + grp) - row[0] * c.kv_heads;
 #pragma unroll
-    for (int u = 0; u < kUnroll; u++) {
+    for (int u = 0; u < U; u++) {
         if (u) {
             row[u] = row[u - 1] + walk.lines;
             kvh[u] = kvh[u - 1] + walk.heads;
@@ -197,7 +278,7 @@ __global__ void __launch_bounds__(kThreads)
         const uint32_t v = v0 + u * GROUPS + grp;
         const bool live = v < walk.total;
         pos[u] = live ? step[row[u]].position : 0xffffffffu;
-        load8(src + (live ? (uint64_t)v * c.head + e0 : 0), live ? left : 0, vec, x[u]);
+        load16(src + (live ? (uint64_t)v * c.head + e0 : 0), live ? left : 0, vec, x[u]);
         if (live && pos[u] >= c.seq && sub == 0) atomicOr(flags, kFlagPositionRange);
     }
     // rows of one cache at the same position: the last one is written. Rising positions (a
@@ -221,27 +302,14 @@ __global__ void __launch_bounds__(kThreads)
         }
         __syncthreads();
 #pragma unroll
-        for (int u = 0; u < kUnroll; u++)
+        for (int u = 0; u < U; u++)
             if (row[u] >= r0 && row[u] < r1 && lost[row[u] - r0]) pos[u] = 0xffffffffu;
     }
     pdl_trigger();
 #pragma unroll
-    for (int u = 0; u < kUnroll; u++) {
-        float lo = x[u][0], hi = x[u][0];  // NaN once a value is
-#pragma unroll
-        for (int i = 1; i < 8; i++) {
-            lo = min_nan(lo, x[u][i]);
-            hi = max_nan(hi, x[u][i]);
-        }
-        if (left == 0) {
-            lo = INFINITY;
-            hi = -INFINITY;
-        }
-#pragma unroll
-        for (int o = LPV / 2; o > 0; o >>= 1) {
-            lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-            hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        }
+    for (int u = 0; u < U; u++) {
+        float lo, hi;
+        extremes<LPV>(x[u], left != 0, &lo, &hi);
         const bf16 mb = __float2bfloat16_rn(lo);
         const float m = __bfloat162float(mb);
         const bf16 sb = __float2bfloat16_rn(__fdiv_rn(fmaxf(__fsub_rn(hi, m), 0.0f), 15.0f));
@@ -249,48 +317,52 @@ __global__ void __launch_bounds__(kThreads)
         // a value of the row, its range or its offset is not finite
         const bool bad = !(isfinite(lo) && isfinite(hi) && isfinite(m) && isfinite(s));
         const bool write = pos[u] < c.seq;
-        uint32_t word = 0;
+        uint32_t word[2] = {0, 0};
         if (!bad && s > 0.0f) {
             const float inv = 1.0f / (15.0f * s);
             bool exactly = s < 0x1p-100f;
-            float near = 0.0f, half[2];
+            if constexpr (sizeof(T) == 2) {
+                const float q = -m * inv, twice = fmaf(q, 30.0f, kMagic) - kMagic;
+                exactly |= (q > 0.0f && q < 1.1f && fmaf(0.5f * twice, s, m) == 0.0f &&
+                            ((int)twice & 1)) ||
+                           (m != 0.0f && fabsf(m) < s * 0x1p-11f);
+            }
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                float k[4];
+            for (int j = 0; j < 2; j++) {
+                float near = 0.0f;
+                // eight codes, each with kMagic's bits above it, as digits of base 16
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float v = x[u][4 * h + i], d = v - m;
-                    const float f = __saturatef(d * inv);
-                    k[i] = fmaf(f, 15.0f, kMagic) - kMagic;
+                for (int i = 7; i >= 0; i--) {
+                    const float d = x[u][j].at(i) - m, f = __saturatef(d * inv);
+                    float k = fmaf(f, 15.0f, kMagic);
                     if constexpr (sizeof(T) == 4) {
-                        near = fmaxf(near, fabsf(fmaf(f, 15.0f, -k[i])));
+                        near = fmaxf(near, fabsf(fmaf(f, 15.0f, kMagic - k)));
                     } else {
                         const float even = fmaf(f, 7.5f, kMagic) - kMagic;
-                        const bool tie = fabsf(fmaf(-k[i], s, d)) == 0.5f * s;
-                        exactly |= tie && d + m != v;
-                        k[i] = tie ? even + even : k[i];
+                        if (fabsf(fmaf(kMagic - k, s, d)) == 0.5f * s) k = fmaf(even, 2.0f, kMagic);
                     }
+                    word[j] = word[j] * 16 + __float_as_uint(k);
                 }
-                // four codes as one whole number below 2^16
-                half[h] = fmaf(fmaf(fmaf(k[3], 16.0f, k[2]), 16.0f, k[1]), 16.0f, k[0]);
+                word[j] -= 0x4b400000u * 0x11111111u;
+                const uint32_t here = left > 8u * j ? left - 8 * j : 0;
+                if ((exactly || near > kNearHalf) && write)
+                    word[j] = exact_word(
+                        src + ((uint64_t)(v0 + u * GROUPS + grp) * c.head + e0 + 8 * j), here, m, s);
+                if (here < 8) word[j] &= here ? 0xffffffffu >> (32 - 4 * here) : 0u;
             }
-            word = (__float_as_uint(half[0] + kMagic) & 0xffffu) |
-                   __float_as_uint(half[1] + kMagic) << 16;
-            if ((exactly || near > kNearHalf) && write)
-                word = exact_word(src + ((uint64_t)(v0 + u * GROUPS + grp) * c.head + e0), left, m, s);
-            if (left < 8) word &= left ? 0xffffffffu >> (32 - 4 * left) : 0u;
         }
         if (!write) continue;
         const uint64_t at = (uint64_t)row[u] * c.row_stride + (uint64_t)kvh[u] * c.seq + pos[u];
-        if (sub < c.words) codes[at * c.words + sub] = word;
+        if (2 * sub < c.words)
+            *reinterpret_cast<uint2*>(codes + at * c.words + 2 * sub) = make_uint2(word[0], word[1]);
         if (sub == 0)
             scales[at] = bad ? 0x7fff7fffu
-                                      : (uint32_t)__bfloat16_as_ushort(sb) |
-                                            ((uint32_t)__bfloat16_as_ushort(mb) << 16);
+                             : (uint32_t)__bfloat16_as_ushort(sb) |
+                                   ((uint32_t)__bfloat16_as_ushort(mb) << 16);
     }
 }
 
-// Reading back: the same lane groups, each lane turning one code word into eight values.
+// Reading back: LPV lanes a vector, each turning one code word into eight values.
 // Output row i of batch row b is position step[b].position + i; positions past the cache's
 // end give zeros and raise the position flag.
 template <typename T, int LPV>
@@ -298,7 +370,7 @@ __global__ void __launch_bounds__(kThreads)
     kv4_load_kernel(T* key, T* value, const Kv4View c, const Walk walk, uint32_t n,
                     const Step* step, int vec, uint32_t* flags) {
     constexpr uint32_t GROUPS = kThreads / LPV;
-    constexpr uint32_t VECS = GROUPS * kUnroll;
+    constexpr uint32_t VECS = GROUPS * kLoadUnroll;
     pdl_wait();
     pdl_trigger();
     const uint32_t which = blockIdx.y;
@@ -310,9 +382,9 @@ __global__ void __launch_bounds__(kThreads)
     const uint32_t v0 = blockIdx.x * VECS + grp;
     uint32_t line = v0 / c.kv_heads, kvh = v0 - line * c.kv_heads;
     uint32_t b = line / n, i = line - b * n;
-    uint32_t word[kUnroll], sc[kUnroll];
+    uint32_t word[kLoadUnroll], sc[kLoadUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; u++) {
+    for (int u = 0; u < kLoadUnroll; u++) {
         word[u] = sc[u] = 0;
         if (v0 + u * GROUPS < walk.total) {
             const uint64_t pos = (uint64_t)step[b].position + i;
@@ -336,7 +408,7 @@ __global__ void __launch_bounds__(kThreads)
         }
     }
 #pragma unroll
-    for (int u = 0; u < kUnroll; u++) {
+    for (int u = 0; u < kLoadUnroll; u++) {
         const uint32_t v = v0 + u * GROUPS;
         if (v >= walk.total || e0 >= c.head) continue;
         const float s = bf16lo(sc[u]), m = bf16hi(sc[u]);
@@ -391,19 +463,22 @@ Kv4Rows rows_of(const ab_tensor& key, const ab_tensor& value, int rank_lo, int r
     return r;
 }
 
+// Calls f with the lanes of a vector of codes, `per` words each.
 template <typename F>
-void with_lanes(uint32_t words, F&& f) {
-    if (words <= 4) f(std::integral_constant<int, 4>());
-    else if (words <= 8) f(std::integral_constant<int, 8>());
+void with_lanes(uint32_t words, int per, F&& f) {
+    const uint32_t lanes = (words + per - 1) / per;
+    if (lanes <= 2) f(std::integral_constant<int, 2>());
+    else if (lanes <= 4) f(std::integral_constant<int, 4>());
+    else if (lanes <= 8) f(std::integral_constant<int, 8>());
     else f(std::integral_constant<int, 16>());
 }
 
-// The walk of rows x kv_heads vectors by groups of `lanes`, and its blocks.
-Walk walk_of(const Kv4Rows& r, int lanes, unsigned* blocks) {
+// The walk of rows x kv_heads vectors by groups of `lanes`, `unroll` each, and its blocks.
+Walk walk_of(const Kv4Rows& r, int lanes, int unroll, unsigned* blocks) {
     const uint64_t total = (uint64_t)r.rows * r.kv_heads;
     if (total >> 31) invalid("parameter `key`: too many vectors for one call");
     const uint32_t groups = kThreads / lanes;
-    *blocks = (unsigned)((total + groups * kUnroll - 1) / (groups * kUnroll));
+    *blocks = (unsigned)((total + groups * unroll - 1) / (groups * unroll));
     return Walk{(uint32_t)total, groups / r.kv_heads, groups % r.kv_heads};
 }
 
@@ -421,8 +496,7 @@ void record_kv4_store(ab_scheme* s, const char* label, ab_tensor key, ab_tensor 
     // settled once instead, by a kernel of its own.
     uint32_t* ordered = nullptr;
     const uint32_t chunks = (r.rows + kRowsPerScan - 1) / kRowsPerScan;
-    const uint64_t block_rows = kThreads * kUnroll / (c.words <= 4 ? 4 : c.words <= 8 ? 8 : 16) /
-                                    r.kv_heads + 2;
+    const uint64_t block_rows = kThreads * 4 / std::max(2u, c.words / 2) / r.kv_heads + 2;
     if (c.row_stride == 0 && r.rows / kThreads * block_rows > 512 && s->rt) {
         s->rt->activate();
         cuda_check(cudaMalloc((void**)&ordered, chunks * 4ull), "cudaMalloc");
@@ -432,20 +506,23 @@ void record_kv4_store(ab_scheme* s, const char* label, ab_tensor key, ab_tensor 
                           r.rows, ordered);
         });
     }
-    with_lanes(c.words, [&](auto lanes) {
+    with_lanes(c.words, 2, [&](auto lanes) {
         constexpr int LPV = decltype(lanes)::value;
-        unsigned blocks = 0;
-        const Walk walk = walk_of(r, LPV, &blocks);
-        auto go = [&](auto tag) {
-            using T = decltype(tag);
-            const T *k = (const T*)key.data, *v = (const T*)value.data;
-            s->add(label, [=](cudaStream_t stream) {
-                return launch(stream, dim3(blocks, 2), dim3(kThreads), 0, true,
-                              kv4_store_kernel<T, LPV>, k, v, c, walk, r.rows, st, r.vec, (const uint32_t*)ordered, flags);
-            });
-        };
-        if (key.dtype == AB_F32) go(float());
-        else go(bf16());
+        if constexpr (LPV <= 8) {
+            auto go = [&](auto tag) {
+                using T = decltype(tag);
+                const T *k = (const T*)key.data, *v = (const T*)value.data;
+                unsigned blocks = 0;
+                const Walk walk = walk_of(r, LPV, kStoreUnroll<T>, &blocks);
+                s->add(label, [=](cudaStream_t stream) {
+                    return launch(stream, dim3(blocks, 2), dim3(kThreads), 0, true,
+                                  kv4_store_kernel<T, LPV>, k, v, c, walk, r.rows, st, r.vec,
+                                  (const uint32_t*)ordered, flags);
+                });
+            };
+            if (key.dtype == AB_F32) go(float());
+            else go(bf16());
+        }
     });
 }
 
@@ -484,10 +561,10 @@ int ab_kernel_kv4_load(ab_scheme* s, const ab_kv4_layer* cache, ab_tensor step, 
         expect_step(step, batch);
         const Step* st = (const Step*)step.data;
         uint32_t* flags = s->rt ? s->rt->flags : nullptr;
-        with_lanes(c.words, [&](auto lanes) {
+        with_lanes(c.words, 1, [&](auto lanes) {
             constexpr int LPV = decltype(lanes)::value;
             unsigned blocks = 0;
-            const Walk walk = walk_of(r, LPV, &blocks);
+            const Walk walk = walk_of(r, LPV, kLoadUnroll, &blocks);
             auto go = [&](auto tag) {
                 using T = decltype(tag);
                 T *k = (T*)key.data, *v = (T*)value.data;
