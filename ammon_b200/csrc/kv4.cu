@@ -11,6 +11,7 @@
 // contiguous run for the attention that streams them.
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "common.cuh"
 #include "internal.h"
@@ -217,12 +218,6 @@ __device__ __noinline__ uint32_t exact_word(const T* p, uint32_t left, float m, 
     return word;
 }
 
-// Vectors go to lane groups in order, kv heads fastest: a group's next one is GROUPS further,
-// `lines` lines and `heads` heads on.
-struct Walk {
-    uint32_t total, lines, heads;
-};
-
 constexpr uint32_t kRowsPerScan = 1024;
 
 // ordered[i]: the rows [1024 i, 1024 (i + 1)] of the parcel are at strictly rising positions.
@@ -236,21 +231,18 @@ __global__ void __launch_bounds__(kRowsPerScan)
     if (threadIdx.x == 0) ordered[blockIdx.x] = all;
 }
 
-// LPV lanes hold one vector, sixteen elements (two code words) each; a block takes U * kThreads /
-// LPV consecutive vectors of one of the two tensors (blockIdx.y), kv heads fastest, so its loads
-// are one contiguous run of the source. All of a lane's loads are issued before the first is
-// used. Bound by instructions (a row of 128: its offset, step and checks once for 16 elements,
-// 12 instructions an element); with eight elements a lane it was half as slow again.
-template <typename T>
-constexpr int kStoreUnroll = sizeof(T) == 2 ? 4 : 2;
+// LPV lanes hold one vector, sixteen elements (two code words) each; a block takes kThreads / LPV
+// consecutive vectors of one of the two tensors (blockIdx.y), kv heads fastest, so its loads are
+// one contiguous run of the source. Bound by instructions, some 24 an element; with eight
+// elements a lane, each vector's own work on twice the lanes, 32768 bf16 rows of 8 x 128 took 88
+// us instead of 79, and with four vectors a lane in flight 79 instead of 66: many blocks of an SM
+// hide the loads better.
 template <typename T, int LPV>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 6)
     kv4_store_kernel(const T* key, const T* value, const Kv4View c,
-                     const Walk walk, uint32_t rows, const Step* step, int vec,
+                     uint32_t total, uint32_t rows, const Step* step, int vec,
                      const uint32_t* ordered, uint32_t* flags) {
-    constexpr int U = kStoreUnroll<T>;
-    constexpr uint32_t GROUPS = kThreads / LPV;
-    constexpr uint32_t VECS = GROUPS * U;
+    constexpr uint32_t VECS = kThreads / LPV;
     __shared__ uint32_t lost[VECS];  // per row of this block: a later row has its position
     pdl_wait();
     const uint32_t which = blockIdx.y;
@@ -261,26 +253,14 @@ __global__ void __launch_bounds__(kThreads)
     const uint32_t sub = threadIdx.x % LPV, grp = threadIdx.x / LPV;
     const uint32_t e0 = sub * 16;
     const uint32_t left = e0 < c.head ? c.head - e0 : 0;
-    Eight<T> x[U][2];
-    uint32_t row[U], kvh[U], pos[U];
-    row[0] = (v0 + grp) / c.kv_heads;
-    kvh[0] = (v0 + grp) - row[0] * c.kv_heads;
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        if (u) {
-            row[u] = row[u - 1] + walk.lines;
-            kvh[u] = kvh[u - 1] + walk.heads;
-            if (kvh[u] >= c.kv_heads) {
-                kvh[u] -= c.kv_heads;
-                row[u]++;
-            }
-        }
-        const uint32_t v = v0 + u * GROUPS + grp;
-        const bool live = v < walk.total;
-        pos[u] = live ? step[row[u]].position : 0xffffffffu;
-        load16(src + (live ? (uint64_t)v * c.head + e0 : 0), live ? left : 0, vec, x[u]);
-        if (live && pos[u] >= c.seq && sub == 0) atomicOr(flags, kFlagPositionRange);
-    }
+    const uint32_t v = v0 + grp;
+    const bool live = v < total;
+    const uint32_t row = live ? v / c.kv_heads : 0, kvh = live ? v - row * c.kv_heads : 0;
+    const T* mine = src + (live ? (uint64_t)v * c.head + e0 : 0);
+    uint32_t pos = live ? step[row].position : 0xffffffffu;
+    Eight<T> x[2];
+    load16(mine, live ? left : 0, vec, x);
+    if (live && pos >= c.seq && sub == 0) atomicOr(flags, kFlagPositionRange);
     // rows of one cache at the same position: the last one is written. Rising positions (a
     // prompt) cannot meet; otherwise the block looks through the rows after its own.
     bool scan = c.row_stride == 0 && rows > 1;
@@ -301,76 +281,122 @@ __global__ void __launch_bounds__(kThreads)
                 if (step[r].position == pq) lost[r - r0] = 1;
         }
         __syncthreads();
-#pragma unroll
-        for (int u = 0; u < U; u++)
-            if (row[u] >= r0 && row[u] < r1 && lost[row[u] - r0]) pos[u] = 0xffffffffu;
+        if (live && lost[row - r0]) pos = 0xffffffffu;
     }
     pdl_trigger();
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        float lo, hi;
-        extremes<LPV>(x[u], left != 0, &lo, &hi);
-        const bf16 mb = __float2bfloat16_rn(lo);
-        const float m = __bfloat162float(mb);
-        const bf16 sb = __float2bfloat16_rn(__fdiv_rn(fmaxf(__fsub_rn(hi, m), 0.0f), 15.0f));
-        const float s = __bfloat162float(sb);
-        // a value of the row, its range or its offset is not finite
-        const bool bad = !(isfinite(lo) && isfinite(hi) && isfinite(m) && isfinite(s));
-        const bool write = pos[u] < c.seq;
-        uint32_t word[2] = {0, 0};
-        if (!bad && s > 0.0f) {
-            const float inv = 1.0f / (15.0f * s);
-            bool exactly = s < 0x1p-100f;
-            if constexpr (sizeof(T) == 2) {
-                const float q = -m * inv, twice = fmaf(q, 30.0f, kMagic) - kMagic;
-                exactly |= (q > 0.0f && q < 1.1f && fmaf(0.5f * twice, s, m) == 0.0f &&
-                            ((int)twice & 1)) ||
-                           (m != 0.0f && fabsf(m) < s * 0x1p-11f);
-            }
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                float near = 0.0f;
-                // eight codes, each with kMagic's bits above it, as digits of base 16
-#pragma unroll
-                for (int i = 7; i >= 0; i--) {
-                    const float d = x[u][j].at(i) - m, f = __saturatef(d * inv);
-                    float k = fmaf(f, 15.0f, kMagic);
-                    if constexpr (sizeof(T) == 4) {
-                        near = fmaxf(near, fabsf(fmaf(f, 15.0f, kMagic - k)));
-                    } else {
-                        const float even = fmaf(f, 7.5f, kMagic) - kMagic;
-                        if (fabsf(fmaf(kMagic - k, s, d)) == 0.5f * s) k = fmaf(even, 2.0f, kMagic);
-                    }
-                    word[j] = word[j] * 16 + __float_as_uint(k);
-                }
-                word[j] -= 0x4b400000u * 0x11111111u;
-                const uint32_t here = left > 8u * j ? left - 8 * j : 0;
-                if ((exactly || near > kNearHalf) && write)
-                    word[j] = exact_word(
-                        src + ((uint64_t)(v0 + u * GROUPS + grp) * c.head + e0 + 8 * j), here, m, s);
-                if (here < 8) word[j] &= here ? 0xffffffffu >> (32 - 4 * here) : 0u;
-            }
+    float lo, hi;
+    extremes<LPV>(x, left != 0, &lo, &hi);
+    const bf16 mb = __float2bfloat16_rn(lo);
+    const float m = __bfloat162float(mb);
+    const bf16 sb = __float2bfloat16_rn(__fdiv_rn(fmaxf(__fsub_rn(hi, m), 0.0f), 15.0f));
+    const float s = __bfloat162float(sb);
+    // a value of the row, its range or its offset is not finite
+    const bool bad = !(isfinite(lo) && isfinite(hi) && isfinite(m) && isfinite(s));
+    const bool write = pos < c.seq;
+    uint32_t word[2] = {0, 0};
+    if (!bad && s > 0.0f) {
+        const float inv = 1.0f / (15.0f * s);
+        bool exactly = s < 0x1p-100f;
+        if constexpr (sizeof(T) == 2) {
+            const float q = -m * inv, twice = fmaf(q, 30.0f, kMagic) - kMagic;
+            exactly |= (q > 0.0f && q < 1.1f && fmaf(0.5f * twice, s, m) == 0.0f &&
+                        ((int)twice & 1)) ||
+                       (m != 0.0f && fabsf(m) < s * 0x1p-11f);
         }
-        if (!write) continue;
-        const uint64_t at = (uint64_t)row[u] * c.row_stride + (uint64_t)kvh[u] * c.seq + pos[u];
-        if (2 * sub < c.words)
-            *reinterpret_cast<uint2*>(codes + at * c.words + 2 * sub) = make_uint2(word[0], word[1]);
-        if (sub == 0)
-            scales[at] = bad ? 0x7fff7fffu
-                             : (uint32_t)__bfloat16_as_ushort(sb) |
-                                   ((uint32_t)__bfloat16_as_ushort(mb) << 16);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            float near = 0.0f;
+            // eight codes, each with kMagic's bits above it, as digits of base 16
+#pragma unroll
+            for (int i = 7; i >= 0; i--) {
+                const float d = x[j].at(i) - m, f = __saturatef(d * inv);
+                float k = fmaf(f, 15.0f, kMagic);
+                if constexpr (sizeof(T) == 4) {
+                    near = fmaxf(near, fabsf(fmaf(f, 15.0f, kMagic - k)));
+                } else {
+                    const float even = fmaf(f, 7.5f, kMagic) - kMagic;
+                    if (fabsf(fmaf(kMagic - k, s, d)) == 0.5f * s) k = fmaf(even, 2.0f, kMagic);
+                }
+                word[j] = word[j] * 16 + __float_as_uint(k);
+            }
+            word[j] -= 0x4b400000u * 0x11111111u;
+            const uint32_t here = left > 8u * j ? left - 8 * j : 0;
+            if ((exactly || near > kNearHalf) && write)
+                word[j] = exact_word(mine + 8 * j, here, m, s);
+            if (here < 8) word[j] &= here ? 0xffffffffu >> (32 - 4 * here) : 0u;
+        }
+    }
+    if (!write) return;
+    const uint64_t at = (uint64_t)row * c.row_stride + (uint64_t)kvh * c.seq + pos;
+    if (2 * sub < c.words)
+        *reinterpret_cast<uint2*>(codes + at * c.words + 2 * sub) = make_uint2(word[0], word[1]);
+    if (sub == 0)
+        scales[at] = bad ? 0x7fff7fffu
+                         : (uint32_t)__bfloat16_as_ushort(sb) |
+                               ((uint32_t)__bfloat16_as_ushort(mb) << 16);
+}
+
+// ---- values ------------------------------------------------------------------------------
+// The eight values of a code word, in order, rounded once to the output's type. A code becomes a
+// number by standing in the low bits of one whose units these are (bf16 128, f32 2^23), which is
+// then taken off; bf16 goes two at a time, elements i and i + 4 of the word.
+__device__ __forceinline__ void values_of(uint32_t word, uint32_t sc, uint32_t (&v)[4]) {
+    const uint32_t s2 = __byte_perm(sc, sc, 0x1010), m2 = __byte_perm(sc, sc, 0x3232);
+    uint32_t p[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const uint32_t x = (word >> (4 * j) & 0x000f000fu) | 0x43004300u;
+        asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(p[j]) : "r"(x), "r"(0x43004300u));
+        asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(p[j]) : "r"(p[j]), "r"(s2), "r"(m2));
+    }
+    v[0] = __byte_perm(p[0], p[1], 0x5410);
+    v[1] = __byte_perm(p[2], p[3], 0x5410);
+    v[2] = __byte_perm(p[0], p[1], 0x7632);
+    v[3] = __byte_perm(p[2], p[3], 0x7632);
+}
+__device__ __forceinline__ void values_of(uint32_t word, uint32_t sc, float (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float x = __uint_as_float((word >> (4 * i) & 15u) | 0x4b000000u);
+        v[i] = fmaf(x - 8388608.0f, bf16lo(sc), bf16hi(sc));
+    }
+}
+// 16 bytes of values, or those of them that the row has (`left`).
+__device__ __forceinline__ void put16(bf16* p, const uint32_t (&v)[4], uint32_t left, bool vec) {
+    if (vec) {
+        *reinterpret_cast<uint4*>(p) = make_uint4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++)
+            if (i < left) p[i] = __ushort_as_bfloat16((unsigned short)(v[i / 2] >> (16 * (i % 2))));
+    }
+}
+__device__ __forceinline__ void put16(float* p, const float (&v)[4], uint32_t left, bool vec) {
+    if (vec) {
+        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++)
+            if (i < left) p[i] = v[i];
     }
 }
 
-// Reading back: LPV lanes a vector, each turning one code word into eight values.
-// Output row i of batch row b is position step[b].position + i; positions past the cache's
-// end give zeros and raise the position flag.
+// Vectors go to lane groups in order, kv heads fastest: a group's next one is GROUPS further,
+// `lines` positions and `heads` heads on.
+struct Walk {
+    uint32_t total, lines, heads;
+};
+
+// Reading back: LPV lanes a vector, 16 bytes of output each (eight bf16 values, a code word, or
+// four f32 values, half of one), so that a warp's stores are whole lines: with eight f32 values a
+// lane, 16 streams of 1000 positions of 12 x 64 took 30 us. Output row i of batch row b is position
+// step[b].position + i; positions past the cache's end give zeros and raise the position flag.
 template <typename T, int LPV>
 __global__ void __launch_bounds__(kThreads)
     kv4_load_kernel(T* key, T* value, const Kv4View c, const Walk walk, uint32_t n,
                     const Step* step, int vec, uint32_t* flags) {
     constexpr uint32_t GROUPS = kThreads / LPV;
-    constexpr uint32_t VECS = GROUPS * kLoadUnroll;
+    constexpr uint32_t PER = 16 / sizeof(T);  // values of a lane
     pdl_wait();
     pdl_trigger();
     const uint32_t which = blockIdx.y;
@@ -378,8 +404,8 @@ __global__ void __launch_bounds__(kThreads)
     const uint32_t* codes = which ? c.codes[1] : c.codes[0];
     const uint32_t* scales = which ? c.scales[1] : c.scales[0];
     const uint32_t sub = threadIdx.x % LPV, grp = threadIdx.x / LPV;
-    const uint32_t e0 = sub * 8;
-    const uint32_t v0 = blockIdx.x * VECS + grp;
+    const uint32_t e0 = sub * PER;
+    const uint32_t v0 = blockIdx.x * (GROUPS * kLoadUnroll) + grp;
     uint32_t line = v0 / c.kv_heads, kvh = v0 - line * c.kv_heads;
     uint32_t b = line / n, i = line - b * n;
     uint32_t word[kLoadUnroll], sc[kLoadUnroll];
@@ -390,7 +416,7 @@ __global__ void __launch_bounds__(kThreads)
             const uint64_t pos = (uint64_t)step[b].position + i;
             if (pos < c.seq) {
                 const uint64_t at = (uint64_t)b * c.row_stride + (uint64_t)kvh * c.seq + pos;
-                if (sub < c.words) word[u] = __ldcg(codes + at * c.words + sub);
+                if (e0 < 8 * c.words) word[u] = __ldcg(codes + at * c.words + e0 / 8) >> 4 * (e0 % 8);
                 sc[u] = __ldcg(scales + at);
             } else if (sub == 0) {
                 atomicOr(flags, kFlagPositionRange);
@@ -411,35 +437,15 @@ __global__ void __launch_bounds__(kThreads)
     for (int u = 0; u < kLoadUnroll; u++) {
         const uint32_t v = v0 + u * GROUPS;
         if (v >= walk.total || e0 >= c.head) continue;
-        const float s = bf16lo(sc[u]), m = bf16hi(sc[u]);
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = fmaf((float)((word[u] >> (4 * i)) & 15u), s, m);
-        T* p = dst + (uint64_t)v * c.head + e0;
-        if (vec) {
-            if constexpr (sizeof(T) == 2) {
-                uint4 r;
-                __nv_bfloat162 h;
-                h = __floats2bfloat162_rn(x[0], x[1]); r.x = *reinterpret_cast<uint32_t*>(&h);
-                h = __floats2bfloat162_rn(x[2], x[3]); r.y = *reinterpret_cast<uint32_t*>(&h);
-                h = __floats2bfloat162_rn(x[4], x[5]); r.z = *reinterpret_cast<uint32_t*>(&h);
-                h = __floats2bfloat162_rn(x[6], x[7]); r.w = *reinterpret_cast<uint32_t*>(&h);
-                *reinterpret_cast<uint4*>(p) = r;
-            } else {
-                reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-                reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
-            }
-        } else {
-#pragma unroll
-            for (uint32_t i = 0; i < 8; i++)
-                if (e0 + i < c.head) p[i] = from_f32<T>(x[i]);
-        }
+        typename std::conditional<sizeof(T) == 2, uint32_t[4], float[4]>::type x;
+        values_of(word[u], sc[u], x);
+        put16(dst + (uint64_t)v * c.head + e0, x, c.head - e0, vec);
     }
 }
 
 // Rows [n, kv_heads, head], or [kv_heads, head] for one; both tensors alike.
 struct Kv4Rows {
-    uint32_t rows, kv_heads, head;
+    uint32_t rows, kv_heads, head, vectors;
     int vec;  // 16-byte accesses: whole groups of eight elements, aligned
 };
 
@@ -457,29 +463,25 @@ Kv4Rows rows_of(const ab_tensor& key, const ab_tensor& value, int rank_lo, int r
     r.head = key.dims[key.rank - 1];
     r.kv_heads = key.dims[key.rank - 2];
     const uint64_t rows = numel(key) / ((uint64_t)r.head * r.kv_heads);
-    if (rows > 0x7fffffffu) invalid("parameter `key`: too many rows");
+    if ((rows * r.kv_heads) >> 31) invalid("parameter `key`: too many vectors for one call");
     r.rows = (uint32_t)rows;
+    r.vectors = r.rows * r.kv_heads;
     r.vec = r.head % 8 == 0 && ((uintptr_t)key.data | (uintptr_t)value.data) % 16 == 0;
     return r;
 }
 
-// Calls f with the lanes of a vector of codes, `per` words each.
+// Calls f with the power of two of lanes that covers a vector.
 template <typename F>
-void with_lanes(uint32_t words, int per, F&& f) {
-    const uint32_t lanes = (words + per - 1) / per;
+void with_lanes(uint32_t lanes, F&& f) {
     if (lanes <= 2) f(std::integral_constant<int, 2>());
     else if (lanes <= 4) f(std::integral_constant<int, 4>());
     else if (lanes <= 8) f(std::integral_constant<int, 8>());
-    else f(std::integral_constant<int, 16>());
+    else if (lanes <= 16) f(std::integral_constant<int, 16>());
+    else f(std::integral_constant<int, 32>());
 }
 
-// The walk of rows x kv_heads vectors by groups of `lanes`, `unroll` each, and its blocks.
-Walk walk_of(const Kv4Rows& r, int lanes, int unroll, unsigned* blocks) {
-    const uint64_t total = (uint64_t)r.rows * r.kv_heads;
-    if (total >> 31) invalid("parameter `key`: too many vectors for one call");
-    const uint32_t groups = kThreads / lanes;
-    *blocks = (unsigned)((total + groups * unroll - 1) / (groups * unroll));
-    return Walk{(uint32_t)total, groups / r.kv_heads, groups % r.kv_heads};
+unsigned blocks_for(uint32_t vectors, uint32_t per_block) {
+    return (unsigned)(((uint64_t)vectors + per_block - 1) / per_block);
 }
 
 }  // namespace
@@ -496,7 +498,7 @@ void record_kv4_store(ab_scheme* s, const char* label, ab_tensor key, ab_tensor 
     // settled once instead, by a kernel of its own.
     uint32_t* ordered = nullptr;
     const uint32_t chunks = (r.rows + kRowsPerScan - 1) / kRowsPerScan;
-    const uint64_t block_rows = kThreads * 4 / std::max(2u, c.words / 2) / r.kv_heads + 2;
+    const uint64_t block_rows = kThreads / std::max(2u, c.words / 2) / r.kv_heads + 2;
     if (c.row_stride == 0 && r.rows / kThreads * block_rows > 512 && s->rt) {
         s->rt->activate();
         cuda_check(cudaMalloc((void**)&ordered, chunks * 4ull), "cudaMalloc");
@@ -506,17 +508,16 @@ void record_kv4_store(ab_scheme* s, const char* label, ab_tensor key, ab_tensor 
                           r.rows, ordered);
         });
     }
-    with_lanes(c.words, 2, [&](auto lanes) {
+    with_lanes(c.words / 2, [&](auto lanes) {
         constexpr int LPV = decltype(lanes)::value;
-        if constexpr (LPV <= 8) {
+        if constexpr (LPV <= 8) {  // 16 words at most
+            const unsigned blocks = blocks_for(r.vectors, kThreads / LPV);
             auto go = [&](auto tag) {
                 using T = decltype(tag);
                 const T *k = (const T*)key.data, *v = (const T*)value.data;
-                unsigned blocks = 0;
-                const Walk walk = walk_of(r, LPV, kStoreUnroll<T>, &blocks);
                 s->add(label, [=](cudaStream_t stream) {
                     return launch(stream, dim3(blocks, 2), dim3(kThreads), 0, true,
-                                  kv4_store_kernel<T, LPV>, k, v, c, walk, r.rows, st, r.vec,
+                                  kv4_store_kernel<T, LPV>, k, v, c, r.vectors, r.rows, st, r.vec,
                                   (const uint32_t*)ordered, flags);
                 });
             };
@@ -561,21 +562,22 @@ int ab_kernel_kv4_load(ab_scheme* s, const ab_kv4_layer* cache, ab_tensor step, 
         expect_step(step, batch);
         const Step* st = (const Step*)step.data;
         uint32_t* flags = s->rt ? s->rt->flags : nullptr;
-        with_lanes(c.words, 1, [&](auto lanes) {
-            constexpr int LPV = decltype(lanes)::value;
-            unsigned blocks = 0;
-            const Walk walk = walk_of(r, LPV, kLoadUnroll, &blocks);
-            auto go = [&](auto tag) {
-                using T = decltype(tag);
-                T *k = (T*)key.data, *v = (T*)value.data;
+        auto go = [&](auto tag) {
+            using T = decltype(tag);
+            T *k = (T*)key.data, *v = (T*)value.data;
+            with_lanes(c.words * sizeof(T) / 2, [&](auto lanes) {
+                constexpr int LPV = decltype(lanes)::value;
+                constexpr uint32_t GROUPS = kThreads / LPV;
+                const unsigned blocks = blocks_for(r.vectors, GROUPS * kLoadUnroll);
+                const Walk walk{r.vectors, GROUPS / r.kv_heads, GROUPS % r.kv_heads};
                 s->add("kv4_load", [=](cudaStream_t stream) {
                     return launch(stream, dim3(blocks, 2), dim3(kThreads), 0, true,
                                   kv4_load_kernel<T, LPV>, k, v, c, walk, n, st, r.vec, flags);
                 });
-            };
-            if (key.dtype == AB_F32) go(float());
-            else go(bf16());
-        });
+            });
+        };
+        if (key.dtype == AB_F32) go(float());
+        else go(bf16());
     });
 }
 
