@@ -224,10 +224,9 @@ struct Line {
     }
 };
 
-// What a block's first warp finds for all: its stretch, the unit at hand (tiles [at, until) of
-// the line) and the part of it that is the block's.
+// What a block's first warp finds for all: a unit (tiles [at, until) of the line) and the
+// positions of it that are the block's.
 struct Span {
-    uint32_t begin, end;
     uint32_t item, nth, kvh, sub, at, until, t_begin, t_end;
 };
 
@@ -288,11 +287,11 @@ struct Unit {
 // Joins the parts of blocks first .. first + n - 1 in that order and writes the unit's rows.
 // The [S][32 W] outputs are COLS groups of four; JG threads share one and take every JG-th part
 // (what is left of the threads rests). A thread joins its parts as an online softmax does, so
-// that weights and values are read in one round, AHEAD parts at a time. so (a region of `stride`
-// floats a warp), sm, sl: the block's shared arrays, free by now.
+// that weights and values are read in one round, AHEAD parts at a time. so, sm, sl: the block's
+// shared arrays, free by now.
 template <int W, uint32_t S, typename OT>
 __device__ __forceinline__ void join_parts(const Unit<W, S, OT>& unit, uint32_t first, uint32_t n,
-                                        uint32_t tid, float* so, uint32_t stride, float (*sm)[S],
+                                        uint32_t tid, float* so, float (*sm)[S],
                                            float (*sl)[S]) {
     constexpr uint32_t PART = S * (32 * W + 2), COLS = S * 8 * W;
     constexpr uint32_t JG = kThreads / COLS;
@@ -332,7 +331,7 @@ __device__ __forceinline__ void join_parts(const Unit<W, S, OT>& unit, uint32_t 
     }
     if constexpr (JG > 1) {
         if (jg < JG) {
-            reinterpret_cast<float4*>(so + jg * stride)[col] = x;
+            reinterpret_cast<float4*>(so)[jg * COLS + col] = x;
             sm[jg][s] = J;  // the same from every thread of a slot
             sl[jg][s] = L;
         }
@@ -340,7 +339,7 @@ __device__ __forceinline__ void join_parts(const Unit<W, S, OT>& unit, uint32_t 
         if (jg == 0) {
 #pragma unroll
             for (uint32_t g = 1; g < JG; g++)
-                join(reinterpret_cast<const float4*>(so + g * stride)[col], sm[g][s], sl[g][s]);
+                join(reinterpret_cast<const float4*>(so)[g * COLS + col], sm[g][s], sl[g][s]);
         }
     }
     if (jg == 0) unit.write(col, x, L);
@@ -356,23 +355,24 @@ __global__ void __launch_bounds__(kThreads, kResident)
     constexpr uint32_t PART = S * (HP + 2);
     constexpr uint32_t M0 = 0x000f000fu, M1 = 0x00f000f0u;
     using St = Stage<W>;
-    constexpr uint32_t RING = kStages * St::BYTES;  // a warp's turns; later its outputs [S][HP]
-    static_assert(S * HP * 4 <= RING && RING % 16 == 0, "outputs fit");
+    constexpr uint32_t RING = kStages * St::BYTES;  // a warp's turns
+    constexpr uint32_t QF = NT * W * 2 * 32;        // operand words (uint2) of a unit's queries
+    static_assert(S <= kWarps, "a warp per slot");
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float s_m[kWarps][S], s_l[kWarps][S];
-    __shared__ float s_jm[S], s_jl[S];
-    __shared__ Slot s_slot[S];
-    __shared__ Span span;
+    __shared__ Slot s_slot[2][S];
+    __shared__ Span s_span[3];
     __shared__ Job s_job[2];
-    __shared__ uint32_t s_scan[kWarps], s_item, s_at, s_jobs;
+    __shared__ uint32_t s_scan[kWarps], s_begin, s_end, s_item, s_at, s_jobs;
 
     const uint32_t tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
     pdl_wait();
     pdl_trigger();
     const uint32_t r = lane / 4, c = lane % 4;
     unsigned char* ring = smem + warp * RING;
-    // the queries' operand columns
-    uint2 (*qf)[32] = reinterpret_cast<uint2 (*)[32]>(smem + kWarps * RING);
+    float* so = reinterpret_cast<float*>(smem + kWarps * RING);  // outputs [kWarps][S][HP]
+    // the queries' operand columns, of this unit and the next
+    uint2* s_q = reinterpret_cast<uint2*>(smem + kWarps * (RING + S * HP * 4));
 
     // ---- this block's stretch of the line --------------------------------------------------
     if (blockIdx.x == 0) {
@@ -400,12 +400,12 @@ __global__ void __launch_bounds__(kThreads, kResident)
         line = Line(total, gridDim.x);
         if (lane == 0) {
             const bool any = blockIdx.x < line.blocks;
-            span.begin = any ? line.begin(blockIdx.x) : total;
-            span.end = any ? line.begin(blockIdx.x + 1) : total;
+            s_begin = any ? line.begin(blockIdx.x) : total;
+            s_end = any ? line.begin(blockIdx.x + 1) : total;
         }
     }
     __syncthreads();
-    const uint32_t begin = span.begin, end = span.end;
+    const uint32_t begin = s_begin, end = s_end;
     if (begin >= end) return;
     uint32_t item = 0, item_at = 0;  // tiles before `item`
     if (p.items > 1) {
@@ -439,138 +439,157 @@ __global__ void __launch_bounds__(kThreads, kResident)
         item_at = s_at;
     }
 
-    uint32_t len = 0, n_tiles = 0, jobs = 0;
+    // The units of the stretch overlap: while one's positions are computed, the next one's place
+    // in the line is found and its queries are read; its first turns are on their way while the
+    // warps' parts are joined.
+    uint32_t len = 0, len1 = 0, n_tiles = 0, jobs = 0;  // len1: of the item after
     if (warp == 0) {
         len = item_length<S>(p, item);
+        len1 = item + 1 < p.items ? item_length<S>(p, item + 1) : 0;
         n_tiles = tiles_of(len);
     }
-    for (uint32_t at = begin; at < end;) {
-        // ---- the unit (item, kv head, slot block) at `at` ---------------------------------
-        if (warp == 0) {
-            while (at - item_at >= n_tiles * p.per_item) {
-                item_at += n_tiles * p.per_item;
-                item++;
-                len = item_length<S>(p, item);
-                n_tiles = tiles_of(len);
-            }
-            const uint32_t nth = (at - item_at) / n_tiles;
-            if (lane == 0) {
-                span.item = item;
-                span.nth = nth;
-                span.sub = nth / p.c.kv_heads;
-                span.kvh = nth - span.sub * p.c.kv_heads;
-                span.at = item_at + nth * n_tiles;
-                span.until = span.at + n_tiles;
-                span.t_begin = (at - span.at) * kTile;
-                span.t_end = min((min(end, span.until) - span.at) * kTile, len);
-            }
+    auto plan = [&](uint32_t at, Span& span) {  // the unit at `at`: the first warp's work
+        while (at - item_at >= n_tiles * p.per_item) {
+            item_at += n_tiles * p.per_item;
+            item++;
+            len = len1;
+            len1 = item + 1 < p.items ? item_length<S>(p, item + 1) : 0;
+            n_tiles = tiles_of(len);
         }
-        __syncthreads();
-        const Unit<W, S, OT> unit{p, span.item, span.kvh, span.sub};
-        const uint32_t t_end = span.t_end;
-        const uint64_t vec0 = (uint64_t)(p.shared ? 0 : unit.item) * p.c.row_stride +
-                              (uint64_t)unit.kvh * p.c.seq;
-
-        const unsigned char* ksrc =
-            (const unsigned char*)p.c.codes[0] + vec0 * ROW + lane * 16;
-        const unsigned char* vsrc =
-            (const unsigned char*)p.c.codes[1] + vec0 * ROW + lane * 16;
-        const uint32_t* kscale = p.c.scales[0] + vec0 + lane;
-        const uint32_t* vscale = p.c.scales[1] + vec0 + lane;
-        // The warp's turn at t into stage i, one group of copies (an empty one past the end).
-        // Chunk lane + 32 j is chunk (lane + 32 j) % W of row (lane + 32 j) / W.
-        auto fetch = [&](uint32_t t, uint32_t i) {
-            const uint32_t to = smem_u32(ring) + i * St::BYTES;
-            const unsigned char* k = ksrc + (uint64_t)t * ROW;
-            const unsigned char* v = vsrc + (uint64_t)t * ROW;
-            auto copy = [&](uint32_t n) {  // of n rows
+        const uint32_t nth = (at - item_at) / n_tiles;
+        if (lane == 0) {
+            span.item = item;
+            span.nth = nth;
+            span.sub = nth / p.c.kv_heads;
+            span.kvh = nth - span.sub * p.c.kv_heads;
+            span.at = item_at + nth * n_tiles;
+            span.until = span.at + n_tiles;
+            span.t_begin = (at - span.at) * kTile;
+            span.t_end = min((min(end, span.until) - span.at) * kTile, len);
+        }
+    };
+    const unsigned char *ksrc, *vsrc;
+    const uint32_t *kscale, *vscale;
+    uint32_t t, t_end, stage = 0;
+    // The warp's turn at t into stage i, one group of copies (an empty one past the end).
+    // Chunk lane + 32 j is chunk (lane + 32 j) % W of row (lane + 32 j) / W.
+    auto fetch = [&](uint32_t t, uint32_t i) {
+        const uint32_t to = smem_u32(ring) + i * St::BYTES;
+        const unsigned char* k = ksrc + (uint64_t)t * ROW;
+        const unsigned char* v = vsrc + (uint64_t)t * ROW;
+        auto copy = [&](uint32_t n) {  // of n rows
 #pragma unroll
-                for (uint32_t j = 0; j < W; j++) {
-                    const uint32_t row = (lane + 32 * j) / W;
-                    const uint32_t at = to + St::place(row, (lane + 32 * j) % W);
-                    const uint32_t size = row < n ? 16 : 0;
-                    copy16(at, k + (size ? j * 512 : 0), size);
-                    copy16(at + St::V, v + (size ? j * 512 : 0), size);
-                }
-                const uint32_t size = lane < n ? 4 : 0;
-                copy4(to + St::KS + 4 * lane, kscale + (size ? t : 0), size);
-                copy4(to + St::VS + 4 * lane, vscale + (size ? t : 0), size);
-            };
-            if (t + kTurn <= t_end) copy(kTurn);
-            else if (t < t_end) copy(t_end - t);
-            copies_commit();
+            for (uint32_t j = 0; j < W; j++) {
+                const uint32_t row = (lane + 32 * j) / W;
+                const uint32_t at = to + St::place(row, (lane + 32 * j) % W);
+                const uint32_t size = row < n ? 16 : 0;
+                copy16(at, k + (size ? j * 512 : 0), size);
+                copy16(at + St::V, v + (size ? j * 512 : 0), size);
+            }
+            const uint32_t size = lane < n ? 4 : 0;
+            copy4(to + St::KS + 4 * lane, kscale + (size ? t : 0), size);
+            copy4(to + St::VS + 4 * lane, vscale + (size ? t : 0), size);
         };
-        uint32_t t = span.t_begin + warp * kTurn;
+        if (t + kTurn <= t_end) copy(kTurn);
+        else if (t < t_end) copy(t_end - t);
+        copies_commit();
+    };
+    auto open = [&](const Span& span) {  // the unit's first turns
+        const uint64_t vec0 = (uint64_t)(p.shared ? 0 : span.item) * p.c.row_stride +
+                              (uint64_t)span.kvh * p.c.seq;
+        ksrc = (const unsigned char*)p.c.codes[0] + vec0 * ROW + lane * 16;
+        vsrc = (const unsigned char*)p.c.codes[1] + vec0 * ROW + lane * 16;
+        kscale = p.c.scales[0] + vec0 + lane;
+        vscale = p.c.scales[1] + vec0 + lane;
+        t_end = span.t_end;
+        t = span.t_begin + warp * kTurn;
 #pragma unroll 1
-        for (uint32_t i = 0; i < kStages; i++) fetch(t + i * kTile, i);
-
-        // ---- queries, times log2(e) / sqrt(head), as operand columns -----------------------
-        // Column 2 (s % 4) of slot s is the whole number next to q 2^e, the next one the rest;
-        // e brings the head's largest |q| to [2^10, 2^11). A lane takes four dims.
-        for (uint32_t s = warp; s < S; s += kWarps) {
-            uint32_t row, head;
-            const bool live = unit.slot(s, &row, &head);
-            const uint32_t d0 = lane * 4, hd = p.c.head;
-            float x[4] = {};
-            if (live && d0 < hd) {
-                const float* src = p.q + ((uint64_t)row * p.heads + head) * hd + d0;
-                if (p.qvec) {
-                    const uint4 a = ld16(src);
-                    x[0] = __uint_as_float(a.x); x[1] = __uint_as_float(a.y);
-                    x[2] = __uint_as_float(a.z); x[3] = __uint_as_float(a.w);
-                } else {
+        for (uint32_t i = 0; i < kStages; i++) fetch(t + i * kTile, (stage + i) % kStages);
+    };
+    // Queries, times log2(e) / sqrt(head), as operand columns: column 2 (s % 4) of slot s is the
+    // whole number next to q 2^e, the next one the rest; e brings the head's largest |q| to
+    // [2^10, 2^11). Warp s takes slot s, a lane four dims.
+    float qx[4];
+    int32_t qlimit = 0;
+    auto read_queries = [&](const Span& span) {
+        if (warp >= S) return;
+        uint32_t row, head;
+        const bool live = Unit<W, S, OT>{p, span.item, span.kvh, span.sub}.slot(warp, &row, &head);
+        const uint32_t d0 = lane * 4, hd = p.c.head;
+        qx[0] = qx[1] = qx[2] = qx[3] = 0.0f;
+        if (live && d0 < hd) {
+            const float* src = p.q + ((uint64_t)row * p.heads + head) * hd + d0;
+            if (p.qvec) {
+                const uint4 a = ld16(src);
+                qx[0] = __uint_as_float(a.x); qx[1] = __uint_as_float(a.y);
+                qx[2] = __uint_as_float(a.z); qx[3] = __uint_as_float(a.w);
+            } else {
 #pragma unroll
-                    for (uint32_t k = 0; k < 4; k++)
-                        if (d0 + k < hd) x[k] = __uint_as_float(ld4(src + k));
-                }
-            }
-            const float unit_scale = kLog2e / sqrtf((float)hd);
-            float top = 0.0f, sum = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                x[k] *= unit_scale;
-                top = fmaxf(top, fabsf(x[k]));
-                sum += x[k];
-            }
-            top = warp_max(top);
-            int e = 10 - ((int)(__float_as_uint(top) >> 23) - 127);
-            e = min(max(e, -100), 100);
-            const float up = __uint_as_float((uint32_t)(e + 127) << 23);
-            float first = 0.0f, rest = 0.0f;
-            const uint32_t word = d0 / 8, col = 2 * (s % 4);
-            __half* dst = reinterpret_cast<__half*>(qf) + (d0 / 4) % 2;
-#pragma unroll
-            for (uint32_t k = 0; k < 4; k++) {
-                const float v = x[k] * up, w = rintf(v);  // the rest is NaN where q is not finite
-                first += w;
-                rest += v - w;
-                if (word < 4 * W) {
-                    // code k of a half word is at bits 4 k: even k as c 2^-24, odd as 16 c 2^-24
-                    const uint32_t at = (((s / 4) * W + word % W) * 2 + k / 2) * 32 + word / W;
-                    const float f = k % 2 ? 0.0625f : 1.0f;
-                    dst[((at + col * 4) * 2 + k % 2) * 2] = __float2half_rn(w * f);
-                    dst[((at + col * 4 + 4) * 2 + k % 2) * 2] = __float2half_rn((v - w) * f);
-                }
-            }
-            sum = warp_sum(sum);
-            first = warp_sum(first);
-            rest = warp_sum(rest);
-            if (lane == 0) {
-                int32_t limit = 0x7fffffff;  // past the last slot: nothing of it is written
-                if (live) {
-                    const uint32_t pos = p.step[row].position;
-                    limit = pos < p.c.seq ? (int32_t)pos : -1;
-                }
-                s_slot[s] = Slot{16777216.0f / up, sum, first * (-8.0f / 16777216.0f),
-                                rest * (-8.0f / 16777216.0f), limit};
+                for (uint32_t k = 0; k < 4; k++)
+                    if (d0 + k < hd) qx[k] = __uint_as_float(ld4(src + k));
             }
         }
-        __syncthreads();
+        // past the last slot: nothing of it is written
+        qlimit = live ? (int32_t)min(p.step[row].position, 0x7fffffffu) : 0x7fffffff;
+        if (live && qlimit >= (int32_t)p.c.seq) qlimit = -1;
+    };
+    auto set_queries = [&](uint2* qf, Slot* slots) {
+        if (warp >= S) return;
+        const float unit_scale = kLog2e / sqrtf((float)p.c.head);
+        float top = 0.0f, sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            qx[k] *= unit_scale;
+            top = fmaxf(top, fabsf(qx[k]));
+            sum += qx[k];
+        }
+        top = warp_max(top);
+        int e = 10 - ((int)(__float_as_uint(top) >> 23) - 127);
+        e = min(max(e, -100), 100);
+        const float up = __uint_as_float((uint32_t)(e + 127) << 23);
+        float first = 0.0f, rest = 0.0f;
+        const uint32_t word = lane / 2, col = 2 * (warp % 4);
+        __half* dst = reinterpret_cast<__half*>(qf) + lane % 2;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) {
+            const float v = qx[k] * up, w = rintf(v);  // the rest is NaN where q is not finite
+            first += w;
+            rest += v - w;
+            if (word < 4 * W) {
+                // code k of a half word is at bits 4 k: even k as c 2^-24, odd as 16 c 2^-24
+                const uint32_t at = (((warp / 4) * W + word % W) * 2 + k / 2) * 32 + word / W;
+                const float f = k % 2 ? 0.0625f : 1.0f;
+                dst[((at + col * 4) * 2 + k % 2) * 2] = __float2half_rn(w * f);
+                dst[((at + col * 4 + 4) * 2 + k % 2) * 2] = __float2half_rn((v - w) * f);
+            }
+        }
+        sum = warp_sum(sum);
+        first = warp_sum(first);
+        rest = warp_sum(rest);
+        if (lane == 0)
+            slots[warp] = Slot{16777216.0f / up, sum, first * (-8.0f / 16777216.0f),
+                               rest * (-8.0f / 16777216.0f), qlimit};
+    };
+
+    if (warp == 0) plan(begin, s_span[0]);
+    __syncthreads();
+    open(s_span[0]);
+    read_queries(s_span[0]);
+    set_queries(s_q, s_slot[0]);
+    for (uint32_t nth = 0;; nth++) {
+        const Span& span = s_span[nth % 3];
+        Span& after = s_span[(nth + 1) % 3];
+        const uint32_t next_at = min(end, span.until);
+        const bool more = next_at < end;
+        if (more && warp == 0) plan(next_at, after);
+        __syncthreads();  // this unit's queries, the next one's place; the last one's outputs are read
+        if (more) read_queries(after);
+        const uint2* qf = s_q + nth % 2 * QF;
         float qscale[NT], qsum[NT], qmid[NT][2];  // of slot c (+ 4 nt)
         int32_t limit[NT], lowest = 0x7fffffff;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            const Slot& q = s_slot[c + 4 * nt];
+            const Slot& q = s_slot[nth % 2][c + 4 * nt];
             qscale[nt] = q.scale;
             qsum[nt] = q.sum;
             qmid[nt][0] = q.first;
@@ -598,7 +617,6 @@ __global__ void __launch_bounds__(kThreads, kResident)
         const uint32_t k_at = W == 4   ? St::place(r, c)
                               : W == 2 ? St::place(r, c / 2) + c % 2 * 8
                                        : r * ROW + c * 4 * W;
-        uint32_t stage = 0;
         for (; t < t_end; t += kTile) {
             copies_wait<kStages - 1>();
             __syncwarp();
@@ -626,7 +644,8 @@ __global__ void __launch_bounds__(kThreads, kResident)
                     const uint32_t y0 = x0 >> 8, y1 = x1 >> 8;
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
-                        const uint2 b0 = qf[(nt * W + w) * 2][lane], b1 = qf[(nt * W + w) * 2 + 1][lane];
+                        const uint2 b0 = qf[(nt * W + w) * 64 + lane],
+                                    b1 = qf[(nt * W + w) * 64 + 32 + lane];
                         mma16816(acc[i][nt], x0 & M0, x1 & M0, x0 & M1, x1 & M1, b0.x, b0.y);
                         mma16816(acc[i][nt], y0 & M0, y1 & M0, y0 & M1, y1 & M1, b1.x, b1.y);
                     }
@@ -731,9 +750,13 @@ __global__ void __launch_bounds__(kThreads, kResident)
             stage = (stage + 1) % kStages;
         }
 
+        if (more) {
+            open(after);
+            set_queries(s_q + (nth + 1) % 2 * QF, s_slot[(nth + 1) % 2]);
+        }
+
         // ---- the warps' parts joined -----------------------------------------------------------
-        __syncwarp();
-        float* mo = reinterpret_cast<float*>(ring);
+        float* mo = so + warp * (S * HP);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -755,42 +778,37 @@ __global__ void __launch_bounds__(kThreads, kResident)
             }
         }
         __syncthreads();
-        static_assert(kWarps <= 32, "a lane per warp");
-        for (uint32_t s = warp; s < S; s += kWarps) {
-            const float m = lane < kWarps ? s_m[lane][s] : -INFINITY;
-            const float J = warp_max(m), a = m == -INFINITY ? 0.0f : ex2(m - J);
-            const float L = warp_sum(lane < kWarps ? s_l[lane][s] * a : 0.0f);
-            if (lane < kWarps) s_m[lane][s] = a;
-            if (lane == 0) {
-                s_jm[s] = J;
-                s_jl[s] = L;
-            }
-        }
-        __syncthreads();
+        const Unit<W, S, OT> unit{p, span.item, span.kvh, span.sub};
         const bool whole = begin <= span.at && span.until <= end;
         // a unit that began in an earlier stretch is this block's first part, else its last
         float* mine = p.part + (uint64_t)(2 * blockIdx.x + (begin <= span.at)) * PART;
-        const float* so = reinterpret_cast<const float*>(smem);
         for (uint32_t i = tid; i < S * HP / 4; i += kThreads) {
             const uint32_t s = i * 4 / HP, d = i * 4 % HP;
+            float J = -INFINITY, L = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) J = fmaxf(J, s_m[w][s]);
             float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int w = 0; w < kWarps; w++) {
-                const float4 v = *reinterpret_cast<const float4*>(so + w * (RING / 4) + s * HP + d);
-                const float a = s_m[w][s];
+                const float4 v = *reinterpret_cast<const float4*>(so + (w * S + s) * HP + d);
+                const float a = s_m[w][s] == -INFINITY ? 0.0f : ex2(s_m[w][s] - J);
+                L = fmaf(s_l[w][s], a, L);
                 x.x = fmaf(v.x, a, x.x);
                 x.y = fmaf(v.y, a, x.y);
                 x.z = fmaf(v.z, a, x.z);
                 x.w = fmaf(v.w, a, x.w);
             }
-            if (whole) unit.write(i, x, s_jl[s]);
-            else __stcg(reinterpret_cast<float4*>(mine) + i, x);
+            if (whole) {
+                unit.write(i, x, L);
+            } else {
+                __stcg(reinterpret_cast<float4*>(mine) + i, x);
+                if (d == 0) {
+                    __stcg(mine + S * HP + s, J);
+                    __stcg(mine + S * HP + S + s, L);
+                }
+            }
         }
         if (!whole) {
-            if (tid < S) {
-                __stcg(mine + S * HP + tid, s_jm[tid]);
-                __stcg(mine + S * HP + S + tid, s_jl[tid]);
-            }
             __syncthreads();  // the block's part is written; its first thread publishes it
             if (tid == 0) {
                 // blocks first .. last meet this unit; the last to arrive joins their parts, after
@@ -804,15 +822,14 @@ __global__ void __launch_bounds__(kThreads, kResident)
                 }
             }
         }
-        at = min(end, span.until);
-        __syncthreads();  // the next unit reuses the shared arrays
+        if (!more) break;
     }
     if (tid == 0) s_jobs = jobs;
     __syncthreads();
     for (uint32_t k = 0; k < s_jobs; k++) {
         const Job& job = s_job[k];
         join_parts<W, S>(Unit<W, S, OT>{p, job.item, job.kvh, job.sub}, job.first, job.parts,
-                         tid, reinterpret_cast<float*>(smem), RING / 4, s_m, s_l);
+                         tid, so, s_m, s_l);
         __syncthreads();
     }
 }
@@ -820,8 +837,8 @@ __global__ void __launch_bounds__(kThreads, kResident)
 template <int W, int NT, typename OT>
 void record_one(ab_scheme* s, Kv4AttnParams p) {
     constexpr uint32_t S = 4 * NT, PART = S * (32 * W + 2);
-    constexpr size_t smem = kWarps * kStages * Stage<W>::BYTES +
-                            NT * W * 2 * 32 * sizeof(uint2);
+    constexpr size_t smem = kWarps * (kStages * Stage<W>::BYTES + S * 32 * W * 4) +
+                            2 * NT * W * 2 * 32 * sizeof(uint2);
     auto* kernel = kv4_attention_kernel<W, NT, OT>;
     s->rt->activate();
     cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
