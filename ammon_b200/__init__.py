@@ -448,6 +448,14 @@ class Kv4Cache:
         self._h = h
         self.rt = rt
 
+    @classmethod
+    def _borrow(cls, rt, handle):
+        obj = cls.__new__(cls)
+        obj._h = handle
+        obj.rt = rt
+        obj._borrowed = True
+        return obj
+
     def layer(self, layer: int) -> Kv4Layer:
         c = _abi.Kv4Layer_t()
         _check(_abi.lib().ab_kv4cache_layer(self._h, layer, C.byref(c)))
@@ -458,9 +466,9 @@ class Kv4Cache:
         _check(_abi.lib().ab_kv4cache_zero(self._h))
 
     def close(self):
-        if getattr(self, "_h", None):
+        if getattr(self, "_h", None) and not getattr(self, "_borrowed", False):
             _abi.lib().ab_kv4cache_destroy(self._h)
-            self._h = None
+        self._h = None
 
     def __del__(self):
         try:
@@ -498,11 +506,16 @@ class CausalAttentionBlock:
         self.rt = rt
 
     def record(self, scheme: Scheme, x: Tensor, weights: CausalAttentionBlockWeights,
-               cache: KvLayer, step: Tensor):
+               cache: "KvLayer | Kv4Layer", step: Tensor):
         w = _abi.AttentionWeights_t(weights.norm.t, weights.query.t, weights.key.t,
                                     weights.value.t, weights.output.t)
-        _check(_abi.lib().ab_attention_block_record(self._h, scheme.handle, x.t, C.byref(w),
-                                                    cache.key.t, cache.value.t, step.t))
+        if isinstance(cache, Kv4Layer):
+            layer = cache.c
+            _check(_abi.lib().ab_attention_block_record_kv4(
+                self._h, scheme.handle, x.t, C.byref(w), C.byref(layer), step.t))
+        else:
+            _check(_abi.lib().ab_attention_block_record(self._h, scheme.handle, x.t, C.byref(w),
+                                                        cache.key.t, cache.value.t, step.t))
         scheme.keep(self, x, weights, cache, step)
 
     def close(self):
@@ -629,14 +642,19 @@ class Comm:
 class LlamaModel:
     """Llama-shaped decode model on the fused kernels (an architecture-crate role the
     reference leaves open, README.md:5,21). ``step`` is AutoregressiveModel::step.
-    With ``comm`` the model is this rank's tensor-parallel shard."""
+    With ``comm`` the model is this rank's tensor-parallel shard; with ``kv4`` it keeps a 4-bit
+    K/V cache."""
 
-    def __init__(self, rt: Runtime, cfg: LlamaConfig, comm: Optional[Comm] = None):
+    def __init__(self, rt: Runtime, cfg: LlamaConfig, comm: Optional[Comm] = None,
+                 kv4: bool = False):
         c = _abi.LlamaConfig_t(cfg.dim, cfg.layers, cfg.heads, cfg.kv_heads, cfg.head_dim,
                                cfg.hidden, cfg.vocab, cfg.seq, cfg.batch, cfg.rope_theta,
                                cfg.norm_eps, cfg.dtype)
         h = C.c_void_p()
-        if comm is None:
+        if kv4:
+            _check(_abi.lib().ab_llama_create_kv4(
+                rt.handle, C.byref(c), comm.handle if comm is not None else None, C.byref(h)))
+        elif comm is None:
             _check(_abi.lib().ab_llama_create(rt.handle, C.byref(c), C.byref(h)))
         else:
             _check(_abi.lib().ab_llama_create_tp(rt.handle, C.byref(c), comm.handle,
@@ -704,6 +722,12 @@ class LlamaModel:
         h = C.c_void_p()
         _check(_abi.lib().ab_llama_cache(self._h, C.byref(h)))
         return KvCache._borrow(self.rt, h)
+
+    def kv4_cache(self) -> Kv4Cache:
+        """The 4-bit cache of a model made with ``kv4``."""
+        h = C.c_void_p()
+        _check(_abi.lib().ab_llama_kv4cache(self._h, C.byref(h)))
+        return Kv4Cache._borrow(self.rt, h)
 
     def reset(self):
         _check(_abi.lib().ab_llama_reset(self._h))

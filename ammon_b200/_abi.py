@@ -126,6 +126,8 @@ SIGNATURES = {
     "ab_kernel_kv4_attention": (C.c_int, [P, T, C.POINTER(Kv4Layer_t), T, T]),
     "ab_attention_block_create": (C.c_int, [P, u32, u32, u32, u32, f32, PP]),
     "ab_attention_block_record": (C.c_int, [P, P, T, C.POINTER(AttentionWeights_t), T, T, T]),
+    "ab_attention_block_record_kv4": (C.c_int, [P, P, T, C.POINTER(AttentionWeights_t),
+                                                C.POINTER(Kv4Layer_t), T]),
     "ab_attention_block_destroy": (C.c_int, [P]),
     "ab_swiglu_block_create": (C.c_int, [P, u32, u32, u32, PP]),
     "ab_swiglu_block_record": (C.c_int, [P, P, T, C.POINTER(SwigluWeights_t)]),
@@ -144,6 +146,8 @@ SIGNATURES = {
     "ab_bpe_decode": (C.c_int, [P, i32, i32, C.c_char_p, u32, C.POINTER(u32)]),
     "ab_bpe_destroy": (C.c_int, [P]),
     "ab_llama_create": (C.c_int, [P, C.POINTER(LlamaConfig_t), PP]),
+    "ab_llama_create_kv4": (C.c_int, [P, C.POINTER(LlamaConfig_t), P, PP]),
+    "ab_llama_kv4cache": (C.c_int, [P, PP]),
     "ab_llama_init_synthetic": (C.c_int, [P, u64, f32]),
     "ab_llama_weight": (C.c_int, [P, i32, u32, C.POINTER(T)]),
     "ab_llama_cache": (C.c_int, [P, PP]),

@@ -11,6 +11,7 @@
 
 #include "common.cuh"
 #include "internal.h"
+#include "kv4.h"
 #include "ops.h"
 
 using namespace ab;
@@ -32,6 +33,7 @@ struct ab_attention_block {
     void* attn_out = nullptr;   // [max_batch, heads * head] (f32 or bf16)
     float* part = nullptr;      // split partials
     uint32_t* counters = nullptr;
+    float* kv_rows = nullptr;  // K and V rows on their way into a 4-bit cache, on first use
     GemmScratch tc;  // tensor-core GEMM scratch (max_batch > kGemvMaxBatch)
     ab_comm* tp = nullptr;   // tensor parallelism: wo output is all-reduced into x
     float* tp_y = nullptr;   // [max_batch, hidden] partial projection
@@ -149,6 +151,204 @@ ab_swiglu_block* swiglu_block_new(ab_runtime* rt, uint32_t hidden, uint32_t inte
 }
 
 }  // namespace ab
+
+namespace {
+
+// Records the block over a cache of f32 or bf16 rows (key, value) or a 4-bit one (cache).
+void record_block(ab_attention_block* blk, ab_scheme* s, ab_tensor x,
+                  const ab_attention_weights* w, const ab_tensor* key_, const ab_tensor* value_,
+                  const ab_kv4_layer* cache, ab_tensor step) {
+    if (!blk || !s || !w) fail(AB_ERR_ARGUMENT, "null argument");
+    const uint32_t hidden = blk->hidden, head = blk->head, heads = blk->heads;
+    const uint32_t qd = heads * head;
+    const uint32_t batch = x_batch(x, hidden, blk->max_batch);
+    expect_data("norm", w->norm);
+    expect_rank("norm", w->norm, 1);
+    expect_float("norm", w->norm);
+    expect_dim("norm", w->norm, 0, "hidden", hidden);
+    const int32_t wdt = w->query.dtype;
+    if (wdt != AB_F32 && wdt != AB_BF16) expect_float("query", w->query);
+    expect_linear("query", w->query, qd, hidden, wdt);
+    expect_linear("key", w->key, 0, hidden, wdt);
+    expect_linear("value", w->value, 0, hidden, wdt);
+    expect_linear("output", w->output, hidden, qd, wdt);
+    const uint32_t kvd = w->key.dims[0];
+    if (w->value.dims[0] != kvd) invalid("attention: wk and wv row counts differ");
+    if (kvd > qd || kvd % 2 != 0)
+        invalid("attention: kv width must be even and no wider than q");
+    if (head > 128) invalid("attention: head size " + std::to_string(head) + " exceeds 128");
+    if (kvd % head) invalid("attention: kv width must be a whole number of heads");
+    const uint32_t kv_heads = kvd / head;
+    int cr = 4;  // rank of the cache views
+    Kv4View c4 = {};
+    if (cache) {
+        c4 = kv4_operands(*cache, batch, kv_heads, head);
+        if (c4.seq != blk->seq)
+            invalid("parameter `cache.key_codes`: seq " + std::to_string(c4.seq) +
+                    " differs from the block's " + std::to_string(blk->seq));
+    } else {
+        // cache views: [B, seq, kv, head] (a cache per batch row) or [seq, kv, head] (one
+        // cache every row reads and appends to: at batch 1, or the consecutive positions of
+        // one sequence -- a prompt -- whose rows must then carry distinct positions)
+        expect_data("key", *key_);
+        expect_data("value", *value_);
+        expect_float("key", *key_);
+        expect_dtype("value", *value_, key_->dtype);
+        cr = key_->rank == 3 ? 3 : 4;
+        expect_rank("key", *key_, cr);
+        expect_rank("value", *value_, cr);
+        const int o = cr - 3;
+        if (cr == 4) {
+            if (key_->dims[0] < batch) expect_dim("key", *key_, 0, "batch", batch);
+        }
+        expect_dim("key", *key_, o + 0, "seq", blk->seq);
+        expect_dim("key", *key_, o + 1, "kv_heads", kv_heads);
+        expect_dim("key", *key_, o + 2, "head", head);
+        for (int a = 0; a < cr; a++)
+            if (value_->dims[a] != key_->dims[a])
+                invalid("parameter `value`: dims must match key " + shape_str(*key_));
+    }
+    expect_step(step, batch);
+    const void* segs[3] = {w->query.data, w->key.data, w->value.data};
+    if (!gemv_fusable(wdt, hidden, segs, 3) || !gemv_fusable(wdt, qd, &w->output.data, 1))
+        invalid("attention: hidden and q widths must be multiples of 8 (bf16) or 4 (f32) "
+                "elements with 16-byte aligned weights");
+    if (!cache && !attention_fusable(heads, kv_heads, head, key_->dtype))
+        invalid("attention: fused path needs query_heads / kv_heads in {1, 2, 4, 8} and "
+                "head * element size a multiple of 16 bytes");
+    if (cache && heads % kv_heads) invalid("attention: kv heads must divide the query heads");
+
+    const uint64_t cache_stride = cr == 3 ? 0 : (uint64_t)blk->seq * kvd;
+    const Step* st = (const Step*)step.data;
+    uint32_t* flags = s->rt ? s->rt->flags : nullptr;
+    const int32_t act = wdt;  // activation dtype feeding the projections
+
+    // 1. norm + QKV + RoPE + cache append
+    GemvParams g = {};
+    g.seg[0] = w->query.data;
+    g.seg[1] = w->key.data;
+    g.seg[2] = w->value.data;
+    g.seg_rows[0] = qd;
+    g.seg_rows[1] = kvd;
+    g.seg_rows[2] = kvd;
+    g.n_rows = qd + 2 * kvd;
+    g.units = g.n_rows / 2;
+    g.K = hidden;
+    g.x = x.data;
+    g.x_dtype = AB_F32;
+    g.x_stride = hidden;
+    g.norm_w = w->norm.data;
+    g.norm_dtype = w->norm.dtype;
+    g.eps = 1e-5f;
+    g.q = blk->q;
+    g.qd = qd;
+    g.kvd = kvd;
+    g.head = head;
+    g.seq = blk->seq;
+    g.theta = blk->theta;
+    if (cache) {
+        // K and V rows [batch, kvd] in f32, which the store quantises into the cache
+        if (!blk->kv_rows)
+            blk->kv_rows = (float*)device_alloc(blk->rt, 2ull * blk->max_batch * qd * 4);
+        g.kcache = blk->kv_rows;
+        g.vcache = blk->kv_rows + (uint64_t)blk->max_batch * qd;
+        g.kv_dtype = AB_F32;
+        g.cache_stride = kvd;
+        g.cache_row = 0;
+    } else {
+        g.kcache = key_->data;
+        g.vcache = value_->data;
+        g.kv_dtype = key_->dtype;
+        g.cache_stride = cache_stride;
+        g.cache_row = kvd;
+    }
+    g.step = st;
+    g.flags = flags;
+    attach_tc_scratch(&g, blk->tc);
+    // validation is complete: nothing below throws a validation error after the
+    // first node is added
+    AttnParams a = {};
+    if (!cache) {
+        const uint32_t nsplit = attention_choose_splits(
+            batch, kv_heads, blk->seq, s->rt ? s->rt->sm_count : 148, blk->nsplit_max);
+        a.q = blk->q;
+        a.kcache = key_->data;
+        a.vcache = value_->data;
+        a.kv_dtype = key_->dtype;
+        a.cache_stride = cache_stride;
+        a.out = blk->attn_out;
+        a.out_dtype = act;
+        a.heads = heads;
+        a.kv_heads = kv_heads;
+        a.head = head;
+        a.seq = blk->seq;
+        a.batch = batch;
+        a.nsplit = nsplit;
+        // a split covers several 64-position tiles: a split pays a partial write and a
+        // share of the fold, which shorter ones do not earn back
+        a.min_chunk = attention_min_chunk();
+        uint64_t floats = 0, counters = 0;
+        attention_scratch_size(batch, heads, head, nsplit, &floats, &counters);
+        a.part_o = blk->part;
+        a.part_ml = blk->part + (uint64_t)batch * heads * nsplit * head;
+        a.part_cap = blk->part_floats;
+        a.counters = blk->counters;
+        a.step = st;
+        a.flags = flags;
+    }
+
+    GemvParams o2 = {};
+    o2.seg[0] = w->output.data;
+    o2.seg_rows[0] = hidden;
+    o2.n_rows = hidden;
+    o2.units = (hidden + 1) / 2;
+    o2.K = qd;
+    o2.x = blk->attn_out;
+    o2.x_dtype = act;
+    o2.x_stride = qd;
+    o2.out = x.data;
+    o2.out_dtype = AB_F32;
+    o2.out_stride = hidden;
+    attach_tc_scratch(&o2, blk->tc);
+
+    const size_t before = s->nodes.size();
+    try {
+        record_gemv(s, "attn_qkv_rope", g, wdt, batch, kProNorm, kEpiQkv);
+        if (cache) {
+            ab_tensor k = {g.kcache, AB_F32, 3, {batch, kv_heads, head, 0}}, v = k;
+            v.data = g.vcache;
+            record_kv4_store(s, "attn_kv4_store", k, v, *cache, step);
+            record_kv4_attention(s, "attn_kv4", blk->q, batch, heads, c4, blk->attn_out, act, st);
+        } else {
+            record_attention(s, "attn_decode", a);
+        }
+        if (blk->tp) {
+            // partial projection of this rank's heads; rank 0 adds the residual, and
+            // the all-reduce sums every rank's part straight into x: over NVLink peer
+            // slots at GEMV batches, else through NCCL
+            o2.out = blk->tp_y;
+            o2.addend = comm_rank(blk->tp) == 0 ? (const float*)x.data : nullptr;
+            if (comm_has_peers(blk->tp) && batch <= kTpPeerMaxRows) {
+                const TpPush tgt = comm_push_target(blk->tp);
+                o2.out = tgt.out;
+                record_gemv(s, "attn_wo_partial", o2, wdt, batch, kProNone, kEpiStore);
+                record_tp_reduce(s, "attn_allreduce", blk->tp, tgt, (float*)x.data,
+                                 batch * hidden);
+            } else {
+                record_gemv(s, "attn_wo_partial", o2, wdt, batch, kProNone, kEpiStore);
+                record_allreduce_f32(s, "attn_allreduce", blk->tp, blk->tp_y,
+                                     (float*)x.data, (size_t)batch * hidden);
+            }
+        } else {
+            record_gemv(s, "attn_wo_residual", o2, wdt, batch, kProNone, kEpiResidual);
+        }
+    } catch (...) {
+        s->nodes.resize(before);
+        throw;
+    }
+}
+
+}  // namespace
 
 extern "C" {
 
@@ -279,164 +479,15 @@ int ab_attention_block_create(ab_runtime* rt, uint32_t hidden, uint32_t query_he
 int ab_attention_block_record(ab_attention_block* blk, ab_scheme* s, ab_tensor x,
                               const ab_attention_weights* w, ab_tensor key, ab_tensor value,
                               ab_tensor step) {
+    return guard([&] { record_block(blk, s, x, w, &key, &value, nullptr, step); });
+}
+
+int ab_attention_block_record_kv4(ab_attention_block* blk, ab_scheme* s, ab_tensor x,
+                                  const ab_attention_weights* w, const ab_kv4_layer* cache,
+                                  ab_tensor step) {
     return guard([&] {
-        if (!blk || !s || !w) fail(AB_ERR_ARGUMENT, "null argument");
-        const uint32_t hidden = blk->hidden, head = blk->head, heads = blk->heads;
-        const uint32_t qd = heads * head;
-        const uint32_t batch = x_batch(x, hidden, blk->max_batch);
-        expect_data("norm", w->norm);
-        expect_rank("norm", w->norm, 1);
-        expect_float("norm", w->norm);
-        expect_dim("norm", w->norm, 0, "hidden", hidden);
-        const int32_t wdt = w->query.dtype;
-        if (wdt != AB_F32 && wdt != AB_BF16) expect_float("query", w->query);
-        expect_linear("query", w->query, qd, hidden, wdt);
-        expect_linear("key", w->key, 0, hidden, wdt);
-        expect_linear("value", w->value, 0, hidden, wdt);
-        expect_linear("output", w->output, hidden, qd, wdt);
-        const uint32_t kvd = w->key.dims[0];
-        if (w->value.dims[0] != kvd) invalid("attention: wk and wv row counts differ");
-        if (kvd > qd || kvd % 2 != 0)
-            invalid("attention: kv width must be even and no wider than q");
-        if (head > 128) invalid("attention: head size " + std::to_string(head) + " exceeds 128");
-        if (kvd % head) invalid("attention: kv width must be a whole number of heads");
-        const uint32_t kv_heads = kvd / head;
-        // cache views: [B, seq, kv, head] (a cache per batch row) or [seq, kv, head] (one
-        // cache every row reads and appends to: at batch 1, or the consecutive positions of
-        // one sequence -- a prompt -- whose rows must then carry distinct positions)
-        expect_data("key", key);
-        expect_data("value", value);
-        expect_float("key", key);
-        expect_dtype("value", value, key.dtype);
-        const int cr = key.rank == 3 ? 3 : 4;
-        expect_rank("key", key, cr);
-        expect_rank("value", value, cr);
-        const int o = cr - 3;
-        if (cr == 4) {
-            if (key.dims[0] < batch) expect_dim("key", key, 0, "batch", batch);
-        }
-        expect_dim("key", key, o + 0, "seq", blk->seq);
-        expect_dim("key", key, o + 1, "kv_heads", kv_heads);
-        expect_dim("key", key, o + 2, "head", head);
-        for (int a = 0; a < cr; a++)
-            if (value.dims[a] != key.dims[a])
-                invalid("parameter `value`: dims must match key " + shape_str(key));
-        expect_step(step, batch);
-        const void* segs[3] = {w->query.data, w->key.data, w->value.data};
-        if (!gemv_fusable(wdt, hidden, segs, 3) || !gemv_fusable(wdt, qd, &w->output.data, 1))
-            invalid("attention: hidden and q widths must be multiples of 8 (bf16) or 4 (f32) "
-                    "elements with 16-byte aligned weights");
-        if (!attention_fusable(heads, kv_heads, head, key.dtype))
-            invalid("attention: fused path needs query_heads / kv_heads in {1, 2, 4, 8} and "
-                    "head * element size a multiple of 16 bytes");
-
-        const uint64_t cache_stride = cr == 3 ? 0 : (uint64_t)blk->seq * kvd;
-        const Step* st = (const Step*)step.data;
-        uint32_t* flags = s->rt ? s->rt->flags : nullptr;
-        const int32_t act = wdt;  // activation dtype feeding the projections
-
-        // 1. norm + QKV + RoPE + cache append
-        GemvParams g = {};
-        g.seg[0] = w->query.data;
-        g.seg[1] = w->key.data;
-        g.seg[2] = w->value.data;
-        g.seg_rows[0] = qd;
-        g.seg_rows[1] = kvd;
-        g.seg_rows[2] = kvd;
-        g.n_rows = qd + 2 * kvd;
-        g.units = g.n_rows / 2;
-        g.K = hidden;
-        g.x = x.data;
-        g.x_dtype = AB_F32;
-        g.x_stride = hidden;
-        g.norm_w = w->norm.data;
-        g.norm_dtype = w->norm.dtype;
-        g.eps = 1e-5f;
-        g.q = blk->q;
-        g.qd = qd;
-        g.kvd = kvd;
-        g.head = head;
-        g.seq = blk->seq;
-        g.theta = blk->theta;
-        g.kcache = key.data;
-        g.vcache = value.data;
-        g.kv_dtype = key.dtype;
-        g.cache_stride = cache_stride;
-        g.step = st;
-        g.flags = flags;
-        attach_tc_scratch(&g, blk->tc);
-        // validation is complete: nothing below throws a validation error after the
-        // first node is added
-        const uint32_t nsplit = attention_choose_splits(
-            batch, kv_heads, blk->seq, s->rt ? s->rt->sm_count : 148, blk->nsplit_max);
-        AttnParams a = {};
-        a.q = blk->q;
-        a.kcache = key.data;
-        a.vcache = value.data;
-        a.kv_dtype = key.dtype;
-        a.cache_stride = cache_stride;
-        a.out = blk->attn_out;
-        a.out_dtype = act;
-        a.heads = heads;
-        a.kv_heads = kv_heads;
-        a.head = head;
-        a.seq = blk->seq;
-        a.batch = batch;
-        a.nsplit = nsplit;
-        // a split covers several 64-position tiles: a split pays a partial write and a
-        // share of the fold, which shorter ones do not earn back
-        a.min_chunk = attention_min_chunk();
-        uint64_t floats = 0, counters = 0;
-        attention_scratch_size(batch, heads, head, nsplit, &floats, &counters);
-        a.part_o = blk->part;
-        a.part_ml = blk->part + (uint64_t)batch * heads * nsplit * head;
-        a.part_cap = blk->part_floats;
-        a.counters = blk->counters;
-        a.step = st;
-        a.flags = flags;
-
-        GemvParams o2 = {};
-        o2.seg[0] = w->output.data;
-        o2.seg_rows[0] = hidden;
-        o2.n_rows = hidden;
-        o2.units = (hidden + 1) / 2;
-        o2.K = qd;
-        o2.x = blk->attn_out;
-        o2.x_dtype = act;
-        o2.x_stride = qd;
-        o2.out = x.data;
-        o2.out_dtype = AB_F32;
-        o2.out_stride = hidden;
-        attach_tc_scratch(&o2, blk->tc);
-
-        const size_t before = s->nodes.size();
-        try {
-            record_gemv(s, "attn_qkv_rope", g, wdt, batch, kProNorm, kEpiQkv);
-            record_attention(s, "attn_decode", a);
-            if (blk->tp) {
-                // partial projection of this rank's heads; rank 0 adds the residual, and
-                // the all-reduce sums every rank's part straight into x: over NVLink peer
-                // slots at GEMV batches, else through NCCL
-                o2.out = blk->tp_y;
-                o2.addend = comm_rank(blk->tp) == 0 ? (const float*)x.data : nullptr;
-                if (comm_has_peers(blk->tp) && batch <= kTpPeerMaxRows) {
-                    const TpPush tgt = comm_push_target(blk->tp);
-                    o2.out = tgt.out;
-                    record_gemv(s, "attn_wo_partial", o2, wdt, batch, kProNone, kEpiStore);
-                    record_tp_reduce(s, "attn_allreduce", blk->tp, tgt, (float*)x.data,
-                                     batch * hidden);
-                } else {
-                    record_gemv(s, "attn_wo_partial", o2, wdt, batch, kProNone, kEpiStore);
-                    record_allreduce_f32(s, "attn_allreduce", blk->tp, blk->tp_y,
-                                         (float*)x.data, (size_t)batch * hidden);
-                }
-            } else {
-                record_gemv(s, "attn_wo_residual", o2, wdt, batch, kProNone, kEpiResidual);
-            }
-        } catch (...) {
-            s->nodes.resize(before);
-            throw;
-        }
+        if (!cache) fail(AB_ERR_ARGUMENT, "null argument");
+        record_block(blk, s, x, w, nullptr, nullptr, cache, step);
     });
 }
 
@@ -449,6 +500,7 @@ int ab_attention_block_destroy(ab_attention_block* b) {
         cudaFree(b->attn_out);
         cudaFree(b->part);
         cudaFree(b->counters);
+        if (b->kv_rows) cudaFree(b->kv_rows);
         if (b->tp_y) cudaFree(b->tp_y);
         free_tc_scratch(&b->tc);
         delete b;

@@ -119,7 +119,7 @@ __device__ __forceinline__ void tc_epilogue_chunk(const GemmTcParams& p, uint32_
             const uint32_t i = r - p.qd;
             float c, s;
             rope_cos_sin(i, p.head, pos, p.theta, &c, &s);
-            const uint64_t o = (uint64_t)b * p.cache_stride + (uint64_t)pos * p.kvd + i;
+            const uint64_t o = (uint64_t)b * p.cache_stride + (uint64_t)pos * p.cache_row + i;
             if (p.kv_dtype == AB_F32) {
                 ((float*)p.kcache)[o] = y0 * c - y1 * s;
                 ((float*)p.kcache)[o + 1] = y0 * s + y1 * c;
@@ -129,7 +129,7 @@ __device__ __forceinline__ void tc_epilogue_chunk(const GemmTcParams& p, uint32_
             }
         } else {
             const uint32_t i = r - p.qd - p.kvd;
-            const uint64_t o = (uint64_t)b * p.cache_stride + (uint64_t)pos * p.kvd + i;
+            const uint64_t o = (uint64_t)b * p.cache_stride + (uint64_t)pos * p.cache_row + i;
             if (p.kv_dtype == AB_F32) {
                 ((float*)p.vcache)[o] = y0;
                 ((float*)p.vcache)[o + 1] = y1;
@@ -615,7 +615,7 @@ __global__ void __launch_bounds__(256) splitk_epilogue_kernel(const GemmTcParams
                 const uint32_t k = r - p.qd;
                 float c, s;
                 rope_cos_sin(k, p.head, pos, p.theta, &c, &s);
-                const uint64_t ko = (uint64_t)col * p.cache_stride + (uint64_t)pos * p.kvd + k;
+                const uint64_t ko = (uint64_t)col * p.cache_stride + (uint64_t)pos * p.cache_row + k;
                 if (p.kv_dtype == AB_F32) {
                     ((float*)p.kcache)[ko] = y0 * c - y1 * s;
                     ((float*)p.kcache)[ko + 1] = y0 * s + y1 * c;
@@ -625,7 +625,7 @@ __global__ void __launch_bounds__(256) splitk_epilogue_kernel(const GemmTcParams
                 }
             } else {
                 const uint32_t k = r - p.qd - p.kvd;
-                const uint64_t vo = (uint64_t)col * p.cache_stride + (uint64_t)pos * p.kvd + k;
+                const uint64_t vo = (uint64_t)col * p.cache_stride + (uint64_t)pos * p.cache_row + k;
                 if (p.kv_dtype == AB_F32) {
                     ((float*)p.vcache)[vo] = y0;
                     ((float*)p.vcache)[vo + 1] = y1;

@@ -270,12 +270,12 @@ __global__ void __launch_bounds__(kGemvThreads, 4) gemv_kernel(const GemvParams 
                 const uint32_t i = r - p.qd;
                 float c, s;
                 rope_cos_sin(i, p.head, pos, p.theta, &c, &s);
-                const uint64_t o = (uint64_t)b * p.cache_stride + (uint64_t)pos * p.kvd + i;
+                const uint64_t o = (uint64_t)b * p.cache_stride + (uint64_t)pos * p.cache_row + i;
                 store_elem(p.kcache, p.kv_dtype, o, y0 * c - y1 * s);
                 store_elem(p.kcache, p.kv_dtype, o + 1, y0 * s + y1 * c);
             } else {
                 const uint32_t i = r - p.qd - p.kvd;
-                const uint64_t o = (uint64_t)b * p.cache_stride + (uint64_t)pos * p.kvd + i;
+                const uint64_t o = (uint64_t)b * p.cache_stride + (uint64_t)pos * p.cache_row + i;
                 store_elem(p.vcache, p.kv_dtype, o, y0);
                 store_elem(p.vcache, p.kv_dtype, o + 1, y1);
             }
@@ -449,6 +449,7 @@ void record_gemv(ab_scheme* s, const char* label, GemvParams p, int32_t wdtype, 
             g.vcache = p.vcache;
             g.kv_dtype = p.kv_dtype;
             g.cache_stride = p.cache_stride;
+            g.cache_row = p.cache_row;
             g.step = p.step;
             g.flags = p.flags;
             record_gemm_tc(s, label, g, wdtype, p.seg, p.seg_rows, nseg, xb, xlo, xs, epi);

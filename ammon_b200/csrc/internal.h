@@ -154,6 +154,13 @@ struct Scheme {
     // device buffers that recorded nodes use and the scheme frees when it is destroyed
     // (kernel entry points that need scratch of their own, e.g. ab_kernel_attention_decode)
     std::vector<void*> owned;
+    // of these, what attention over a 4-bit cache shares among its nodes (kv4_attention.cu)
+    struct {
+        void* part = nullptr;
+        uint64_t part_bytes = 0;
+        uint32_t* tickets = nullptr;
+        uint64_t tickets_n = 0;
+    } kv4;
     void add(const char* label, LaunchFn fn) {
         nodes.push_back(Node{label, std::move(fn), FoldInfo{}});
         dirty = true;

@@ -5,6 +5,8 @@
 
 namespace ab {
 
+struct Step;
+
 constexpr uint32_t kKv4MaxHead = 128;
 
 // 32-bit words of one vector's codes: eight elements a word, rows padded to 16 bytes.
@@ -25,5 +27,9 @@ Kv4View kv4_operands(const ab_kv4_layer& c, uint32_t rows, uint32_t kv_heads, ui
 // Quantises rows key/value [rows, kv_heads, head] into the cache at step[row].position.
 void record_kv4_store(ab_scheme* s, const char* label, ab_tensor key, ab_tensor value,
                       const ab_kv4_layer& cache, ab_tensor step);
+// Attention of q [rows, heads, head] over a checked layer's positions 0 .. step[row].position.
+void record_kv4_attention(ab_scheme* s, const char* label, const float* q, uint32_t rows,
+                          uint32_t heads, const Kv4View& cache, void* out, int32_t out_dtype,
+                          const Step* step);
 
 }  // namespace ab

@@ -834,34 +834,51 @@ __global__ void __launch_bounds__(kThreads, kResident)
     }
 }
 
+// The scheme's scratch for parts and tickets (zero between launches). Its nodes run one after
+// the other, so they share it; a node that needs more makes it anew for itself and later ones.
+void take_scratch(ab_scheme* s, uint64_t part_bytes, uint64_t tickets, Kv4AttnParams* p) {
+    auto& have = s->kv4;
+    if (have.part_bytes < part_bytes) {
+        void* d = nullptr;
+        cuda_check(cudaMalloc(&d, part_bytes), "cudaMalloc");
+        s->owned.push_back(d);
+        have.part = d;
+        have.part_bytes = part_bytes;
+    }
+    if (have.tickets_n < tickets) {
+        void* d = nullptr;
+        cuda_check(cudaMalloc(&d, tickets * 4), "cudaMalloc");
+        s->owned.push_back(d);
+        cuda_check(clear_device(s->rt, d, tickets * 4), "clear tickets");
+        have.tickets = (uint32_t*)d;
+        have.tickets_n = tickets;
+    }
+    p->part = (float*)have.part;
+    p->tickets = have.tickets;
+}
+
 template <int W, int NT, typename OT>
-void record_one(ab_scheme* s, Kv4AttnParams p) {
+void record_one(ab_scheme* s, const char* label, Kv4AttnParams p) {
     constexpr uint32_t S = 4 * NT, PART = S * (32 * W + 2);
     constexpr size_t smem = kWarps * (kStages * Stage<W>::BYTES + S * 32 * W * 4) +
                             2 * NT * W * 2 * 32 * sizeof(uint2);
     auto* kernel = kv4_attention_kernel<W, NT, OT>;
-    s->rt->activate();
-    cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
-               "kv4_attention shared memory");
     const uint64_t units = (uint64_t)p.items * p.per_item;
     const uint64_t tiles = units * ((p.c.seq + kTile - 1) / kTile);
     if (tiles >> 31) invalid("kv4_attention: too much work for one call");
-    const uint32_t grid = (uint32_t)std::min<uint64_t>(
-        (uint64_t)s->rt->sm_count * kResident, tiles);
-    const uint64_t part_bytes = (uint64_t)grid * 2 * PART * 4;
-    unsigned char* scratch = nullptr;
-    cuda_check(cudaMalloc((void**)&scratch, part_bytes + units * 4), "cudaMalloc");
-    s->owned.push_back(scratch);
-    cuda_check(clear_device(s->rt, scratch + part_bytes, units * 4), "clear tickets");
-    p.part = (float*)scratch;
-    p.tickets = (uint32_t*)(scratch + part_bytes);
-    s->add("kv4_attention", [=](cudaStream_t stream) {
+    s->rt->activate();
+    cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+               "kv4_attention shared memory");
+    const uint32_t grid =
+        (uint32_t)std::min<uint64_t>((uint64_t)s->rt->sm_count * kResident, tiles);
+    take_scratch(s, (uint64_t)grid * 2 * PART * 4, units, &p);
+    s->add(label, [=](cudaStream_t stream) {
         return launch(stream, dim3(grid), dim3(kThreads), smem, true, kernel, p);
     });
 }
 
 template <int W>
-void record_width(ab_scheme* s, Kv4AttnParams p, int32_t out_dtype) {
+void record_width(ab_scheme* s, const char* label, Kv4AttnParams p, int32_t out_dtype) {
     // four query slots a unit where a kv head has no more, else eight
     p.shared = p.c.row_stride == 0 && p.rows > 1;
     const uint64_t slots = p.shared ? (uint64_t)p.rows * p.group : p.group;
@@ -870,11 +887,43 @@ void record_width(ab_scheme* s, Kv4AttnParams p, int32_t out_dtype) {
     p.items = p.shared ? blocks : p.rows;
     p.per_item = p.c.kv_heads * (p.shared ? 1 : blocks);
     const bool f32 = out_dtype == AB_F32;
-    if (S == 4) f32 ? record_one<W, 1, float>(s, p) : record_one<W, 1, bf16>(s, p);
-    else f32 ? record_one<W, 2, float>(s, p) : record_one<W, 2, bf16>(s, p);
+    if (S == 4)
+        f32 ? record_one<W, 1, float>(s, label, p) : record_one<W, 1, bf16>(s, label, p);
+    else
+        f32 ? record_one<W, 2, float>(s, label, p) : record_one<W, 2, bf16>(s, label, p);
 }
 
 }  // namespace
+
+void record_kv4_attention(ab_scheme* s, const char* label, const float* q, uint32_t rows,
+                          uint32_t heads, const Kv4View& cache, void* out, int32_t out_dtype,
+                          const Step* step) {
+    const uint32_t head = cache.head;
+    if ((uint64_t)rows * heads > 1u << 30) invalid("parameter `q`: too many rows");
+    if (cache.seq > 0x7fffff00u) invalid("parameter `cache.key_codes`: seq exceeds 2^31 - 256");
+    if ((uintptr_t)q % 4 || (uintptr_t)out % dtype_size(out_dtype))
+        invalid("parameter `q` / `out`: not aligned to its elements");
+    if (!s->rt)
+        fail(AB_ERR_ARGUMENT, "kv4_attention: the scheme needs a runtime (it allocates the split "
+                              "scratch)");
+    Kv4AttnParams p = {};
+    p.c = cache;
+    p.q = q;
+    p.out = out;
+    p.rows = rows;
+    p.heads = heads;
+    p.group = heads / cache.kv_heads;
+    p.qvec = head % 4 == 0 && (uintptr_t)q % 16 == 0;
+    p.ovec = head % 4 == 0 && (uintptr_t)out % (4 * dtype_size(out_dtype)) == 0;
+    p.step = step;
+    p.flags = s->rt->flags;
+    switch (cache.words / 4) {
+        case 1: record_width<1>(s, label, p, out_dtype); break;
+        case 2: record_width<2>(s, label, p, out_dtype); break;
+        case 3: record_width<3>(s, label, p, out_dtype); break;
+        default: record_width<4>(s, label, p, out_dtype); break;
+    }
+}
 
 }  // namespace ab
 
@@ -897,34 +946,13 @@ extern "C" int ab_kernel_kv4_attention(ab_scheme* s, ab_tensor q, const ab_kv4_l
         if (heads % kv)
             invalid("parameter `cache.key_codes`: kv_heads " + std::to_string(kv) +
                     " must divide the " + std::to_string(heads) + " query heads");
-        Kv4AttnParams p = {};
-        p.c = kv4_operands(*cache, rows, kv, head);
+        const Kv4View c = kv4_operands(*cache, rows, kv, head);
         if (numel(out) != (uint64_t)rows * heads * head)
             invalid("parameter `out`: expected " +
                     std::to_string((uint64_t)rows * heads * head) +
                     " elements ([batch, heads * head]), got " + shape_str(out));
         expect_step(step, rows);
-        if ((uint64_t)rows * heads > 1u << 30) invalid("parameter `q`: too many rows");
-        if (p.c.seq > 0x7fffff00u) invalid("parameter `cache.key_codes`: seq exceeds 2^31 - 256");
-        if ((uintptr_t)q.data % 4 || (uintptr_t)out.data % dtype_size(out.dtype))
-            invalid("parameter `q` / `out`: not aligned to its elements");
-        if (!s->rt)
-            fail(AB_ERR_ARGUMENT, "kv4_attention: the scheme needs a runtime (it allocates the "
-                                  "split scratch)");
-        p.q = (const float*)q.data;
-        p.out = out.data;
-        p.rows = rows;
-        p.heads = heads;
-        p.group = heads / kv;
-        p.qvec = head % 4 == 0 && (uintptr_t)q.data % 16 == 0;
-        p.ovec = head % 4 == 0 && (uintptr_t)out.data % (4 * dtype_size(out.dtype)) == 0;
-        p.step = (const Step*)step.data;
-        p.flags = s->rt->flags;
-        switch (p.c.words / 4) {
-            case 1: record_width<1>(s, p, out.dtype); break;
-            case 2: record_width<2>(s, p, out.dtype); break;
-            case 3: record_width<3>(s, p, out.dtype); break;
-            default: record_width<4>(s, p, out.dtype); break;
-        }
+        record_kv4_attention(s, "kv4_attention", (const float*)q.data, rows, heads, c, out.data,
+                             out.dtype, (const Step*)step.data);
     });
 }

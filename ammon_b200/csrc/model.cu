@@ -189,7 +189,8 @@ struct ab_llama {
     uint32_t heads_l = 0, kv_l = 0, hidden_l = 0, vocab_l = 0;  // this rank's shard
     ab_tensor embed = {}, wcls = {}, rms_final = {};
     std::vector<ab_tensor> rms_att, wq, wk, wv, wo, rms_ffn, w1, w2, w3;
-    ab_kvcache* cache = nullptr;
+    ab_kvcache* cache = nullptr;    // one of the two
+    ab_kv4cache* cache4 = nullptr;
     ab_attention_block* attn = nullptr;
     ab_swiglu_block* ffn = nullptr;
     ab_tensor x = {}, logits = {}, step = {}, argmax = {}, history = {};
@@ -277,6 +278,7 @@ void destroy_model(ab_llama* m) {
     if (m->attn) ab_attention_block_destroy(m->attn);
     if (m->ffn) ab_swiglu_block_destroy(m->ffn);
     if (m->cache) ab_kvcache_destroy(m->cache);
+    if (m->cache4) ab_kv4cache_destroy(m->cache4);
     for (auto* v : {&m->rms_att, &m->wq, &m->wk, &m->wv, &m->wo, &m->rms_ffn, &m->w1, &m->w2,
                     &m->w3})
         for (auto& t : *v) free_t(t);
@@ -305,6 +307,19 @@ ab_tensor stream_view(ab_tensor t, uint32_t stream) {
     return t;
 }
 
+// One cache stream's view of a layer of the 4-bit cache.
+ab_kv4_layer stream_view(ab_kv4_layer c, uint32_t stream) {
+    for (ab_tensor* t : {&c.key_codes, &c.key_scales, &c.value_codes, &c.value_scales}) {
+        const bool codes = t == &c.key_codes || t == &c.value_codes;
+        if (t->rank == (codes ? 3 : 2)) continue;  // a single stream
+        const uint64_t per = numel(*t) / t->dims[0];
+        t->data = (char*)t->data + stream * per * dtype_size(t->dtype);
+        t->rank--;
+        for (int a = 0; a < t->rank; a++) t->dims[a] = t->dims[a + 1];
+    }
+    return c;
+}
+
 // The embedding and every layer over the rows of x with the DecodeSteps of `step`. Each row
 // appends to and attends over its own cache stream, or, with stream >= 0, every row is a
 // position of that one stream (a prompt's consecutive positions).
@@ -318,14 +333,21 @@ void record_layers(ab_llama* m, ab_scheme* s, ab_tensor x, ab_tensor step,
     }
     check(ab_embedding_record(s, m->embed, step, x));
     for (uint32_t l = 0; l < c.layers; l++) {
-        ab_tensor key, value;
-        check(ab_kvcache_layer(m->cache, l, &key, &value));
-        if (stream >= 0) {
-            key = stream_view(key, (uint32_t)stream);
-            value = stream_view(value, (uint32_t)stream);
-        }
         ab_attention_weights aw = {m->rms_att[l], m->wq[l], m->wk[l], m->wv[l], m->wo[l]};
-        check(ab_attention_block_record(attn, s, x, &aw, key, value, step));
+        if (m->cache4) {
+            ab_kv4_layer layer;
+            check(ab_kv4cache_layer(m->cache4, l, &layer));
+            if (stream >= 0) layer = stream_view(layer, (uint32_t)stream);
+            check(ab_attention_block_record_kv4(attn, s, x, &aw, &layer, step));
+        } else {
+            ab_tensor key, value;
+            check(ab_kvcache_layer(m->cache, l, &key, &value));
+            if (stream >= 0) {
+                key = stream_view(key, (uint32_t)stream);
+                value = stream_view(value, (uint32_t)stream);
+            }
+            check(ab_attention_block_record(attn, s, x, &aw, key, value, step));
+        }
         ab_swiglu_weights fw = {m->rms_ffn[l], m->w1[l], m->w3[l], m->w2[l]};
         check(ab_swiglu_block_record(ffn, s, x, &fw));
     }
@@ -545,7 +567,8 @@ int vt_step(void* self, uint32_t token, uint32_t pos, const float** logits) {
 uint32_t vt_vocab(void* self) { return ((ab_llama*)self)->c.vocab; }
 uint32_t vt_seq(void* self) { return ((ab_llama*)self)->c.seq; }
 
-ab_llama* create_model(ab_runtime* rt, const ab_llama_config* cfg, ab_comm* comm) {
+ab_llama* create_model(ab_runtime* rt, const ab_llama_config* cfg, ab_comm* comm,
+                       bool kv4 = false) {
     if (!rt || !cfg) fail(AB_ERR_ARGUMENT, "null argument");
     const ab_llama_config c = *cfg;
     if (!c.dim || !c.layers || !c.heads || !c.kv_heads || !c.head_dim || !c.hidden || !c.vocab ||
@@ -585,7 +608,11 @@ ab_llama* create_model(ab_runtime* rt, const ab_llama_config* cfg, ab_comm* comm
             m->w2.push_back(alloc_t(rt, dt, {c.dim, m->hidden_l}));
             m->w3.push_back(alloc_t(rt, dt, {m->hidden_l, c.dim}));
         }
-        check(ab_kvcache_create(rt, c.layers, c.seq, m->kv_l, c.head_dim, dt, c.batch, &m->cache));
+        if (kv4)
+            check(ab_kv4cache_create(rt, c.layers, c.seq, m->kv_l, c.head_dim, c.batch, &m->cache4));
+        else
+            check(ab_kvcache_create(rt, c.layers, c.seq, m->kv_l, c.head_dim, dt, c.batch,
+                                    &m->cache));
         // NVLink peer slots for the per-block row all-reduce. That path carries at most
         // kTpPeerMaxRows rows (wider steps and prefill passes take NCCL), so the slots depend
         // on the width alone and every model of this width on the communicator shares them
@@ -615,7 +642,7 @@ ab_llama* create_model(ab_runtime* rt, const ab_llama_config* cfg, ab_comm* comm
                    "pinned steps");
         check(ab_scheme_create(rt, &m->scheme));
         check(ab_scheme_create(rt, &m->loop_scheme));
-        if (fused_step_enabled()) {
+        if (fused_step_enabled() && !kv4) {
             // this rank's shard; every rank reaches the same decision (same config and
             // environment), so the collective exchange-block set-up is entered by all or none
             FusedStepModel fm;
@@ -747,6 +774,14 @@ int ab_llama_create_tp(ab_runtime* rt, const ab_llama_config* cfg, ab_comm* comm
     });
 }
 
+int ab_llama_create_kv4(ab_runtime* rt, const ab_llama_config* cfg, ab_comm* comm,
+                        ab_llama** out) {
+    return guard([&] {
+        if (!out) fail(AB_ERR_ARGUMENT, "null argument");
+        *out = create_model(rt, cfg, comm, true);
+    });
+}
+
 int ab_llama_init_synthetic(ab_llama* m, uint64_t seed, float std) {
     return guard([&] {
         if (!m) fail(AB_ERR_ARGUMENT, "null model");
@@ -810,7 +845,16 @@ int ab_llama_weight(ab_llama* m, int32_t which, uint32_t layer, ab_tensor* out) 
 int ab_llama_cache(ab_llama* m, ab_kvcache** out) {
     return guard([&] {
         if (!m || !out) fail(AB_ERR_ARGUMENT, "null argument");
+        if (!m->cache) fail(AB_ERR_ARGUMENT, "the model keeps a 4-bit cache (ab_llama_kv4cache)");
         *out = m->cache;
+    });
+}
+
+int ab_llama_kv4cache(ab_llama* m, ab_kv4cache** out) {
+    return guard([&] {
+        if (!m || !out) fail(AB_ERR_ARGUMENT, "null argument");
+        if (!m->cache4) fail(AB_ERR_ARGUMENT, "the model keeps no 4-bit cache (ab_llama_cache)");
+        *out = m->cache4;
     });
 }
 
@@ -1114,7 +1158,7 @@ int ab_llama_logits(ab_llama* m, ab_tensor* out) {
 int ab_llama_reset(ab_llama* m) {
     return guard([&] {
         if (!m) fail(AB_ERR_ARGUMENT, "null model");
-        check(ab_kvcache_zero(m->cache));
+        check(m->cache4 ? ab_kv4cache_zero(m->cache4) : ab_kvcache_zero(m->cache));
         m->rt->activate();
         cuda_check(cudaStreamSynchronize(m->rt->stream), "reset synchronize");
     });

@@ -75,6 +75,7 @@ struct GemvParams {
     void* vcache;
     int32_t kv_dtype;
     uint64_t cache_stride;  // elements between consecutive batch rows of the cache
+    uint32_t cache_row;     // elements between positions (0: rows [batch, kvd], no positions)
     const Step* step;
     uint32_t* flags;
     // scratch for the tensor-core path at batch > 4; null = GEMV only
@@ -117,6 +118,7 @@ struct GemmTcParams {
     void* vcache;
     int32_t kv_dtype;
     uint64_t cache_stride;
+    uint32_t cache_row;
     const Step* step;
     uint32_t* flags;
 };

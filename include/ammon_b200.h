@@ -68,6 +68,7 @@ typedef struct ab_kvcache ab_kvcache;
 typedef struct ab_attention_block ab_attention_block;
 typedef struct ab_swiglu_block ab_swiglu_block;
 typedef struct ab_llama ab_llama;
+typedef struct ab_comm ab_comm;
 
 /* ---- runtime (src/gpu.rs:5-13 create_runtime) ---------------------------- */
 int ab_runtime_create(int32_t device, ab_runtime** out);
@@ -266,6 +267,14 @@ int ab_attention_block_create(ab_runtime* rt, uint32_t hidden, uint32_t query_he
 int ab_attention_block_record(ab_attention_block* b, ab_scheme* s, ab_tensor x,
                               const ab_attention_weights* w, ab_tensor key, ab_tensor value,
                               ab_tensor step);
+/* The block over a 4-bit cache (no counterpart in the reference): K and V rows come out of the
+ * projection in f32, rotated, are quantised into the cache at step.position (ab_kernel_kv4_store)
+ * and attended over there (ab_kernel_kv4_attention), so every token, the row's own included, is
+ * seen as the cache holds it. cache: a cache per row of x, or one that all rows share; its seq is
+ * the block's. Any whole number of query heads per kv head. */
+int ab_attention_block_record_kv4(ab_attention_block* b, ab_scheme* s, ab_tensor x,
+                                  const ab_attention_weights* w, const ab_kv4_layer* cache,
+                                  ab_tensor step);
 int ab_attention_block_destroy(ab_attention_block* b);
 
 /* SwiGluBlockWeights (src/modules.rs:23-28): gate = w1, up = w3, down = w2. */
@@ -363,6 +372,12 @@ typedef struct {
 } ab_llama_config;
 
 int ab_llama_create(ab_runtime* rt, const ab_llama_config* cfg, ab_llama** out);
+/* The model with a 4-bit K/V cache instead of one of cfg's dtype: about 0.53 bytes a value at
+ * head_dim 128. Steps, prefill and generation as with ab_llama_create (or, with a communicator,
+ * ab_llama_create_tp; comm may be NULL); the step runs as its graph of kernels, not as the
+ * persistent launch. head_dim 1..128 with whole query heads per kv head. */
+int ab_llama_create_kv4(ab_runtime* rt, const ab_llama_config* cfg, ab_comm* comm,
+                        ab_llama** out);
 /* Seeded synthetic weights, the same streams the CPU oracle uses. */
 int ab_llama_init_synthetic(ab_llama* m, uint64_t seed, float std);
 /* Weight view: which = 0 embed, 1 wcls, 2 rms_final, 3 rms_att, 4 wq, 5 wk, 6 wv, 7 wo,
@@ -370,6 +385,8 @@ int ab_llama_init_synthetic(ab_llama* m, uint64_t seed, float std);
 int ab_llama_weight(ab_llama* m, int32_t which, uint32_t layer, ab_tensor* out);
 /* KV cache of the model (for inspection). */
 int ab_llama_cache(ab_llama* m, ab_kvcache** out);
+/* The 4-bit cache of a model made by ab_llama_create_kv4. */
+int ab_llama_kv4cache(ab_llama* m, ab_kv4cache** out);
 /* One batched decode step: deposits n = batch steps and replays the step graph.
  * logits_host (may be NULL) receives [batch, vocab] fp32; argmax_host (may be NULL)
  * receives [batch] ids from the device argmax (same tie rule as sample_argmax). */
@@ -435,7 +452,6 @@ int ab_llama_destroy(ab_llama* m);
  * communicator wraps NCCL, loaded at run time (the process's already-loaded
  * libnccl.so.2 when there is one). Collectives are recorded into schemes and captured
  * into the step graph like kernels. */
-typedef struct ab_comm ab_comm;
 #define AB_COMM_ID_BYTES 128
 /* A fresh communicator id (rank 0 makes it and shares it with the other ranks). */
 int ab_comm_unique_id(uint8_t* id);

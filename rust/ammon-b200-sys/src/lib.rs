@@ -161,6 +161,7 @@ extern "C" {
     pub fn ab_kernel_kv4_attention(s: *mut ab_scheme, q: ab_tensor, cache: *const ab_kv4_layer, out_: ab_tensor, step: ab_tensor) -> c_int;
     pub fn ab_attention_block_create(rt: *mut ab_runtime, hidden: u32, query_heads: u32, seq_len: u32, max_batch: u32, rope_theta: f32, out_: *mut *mut ab_attention_block) -> c_int;
     pub fn ab_attention_block_record(b: *mut ab_attention_block, s: *mut ab_scheme, x: ab_tensor, w: *const ab_attention_weights, key: ab_tensor, value: ab_tensor, step: ab_tensor) -> c_int;
+    pub fn ab_attention_block_record_kv4(b: *mut ab_attention_block, s: *mut ab_scheme, x: ab_tensor, w: *const ab_attention_weights, cache: *const ab_kv4_layer, step: ab_tensor) -> c_int;
     pub fn ab_attention_block_destroy(b: *mut ab_attention_block) -> c_int;
     pub fn ab_swiglu_block_create(rt: *mut ab_runtime, hidden: u32, intermediate: u32, max_batch: u32, out_: *mut *mut ab_swiglu_block) -> c_int;
     pub fn ab_swiglu_block_record(b: *mut ab_swiglu_block, s: *mut ab_scheme, x: ab_tensor, w: *const ab_swiglu_weights) -> c_int;
@@ -176,6 +177,8 @@ extern "C" {
     pub fn ab_bpe_decode(t: *const ab_bpe, prev_token: i32, token: i32, out_: *mut c_char, cap: u32, n_out: *mut u32) -> c_int;
     pub fn ab_bpe_destroy(t: *mut ab_bpe) -> c_int;
     pub fn ab_llama_create(rt: *mut ab_runtime, cfg: *const ab_llama_config, out_: *mut *mut ab_llama) -> c_int;
+    pub fn ab_llama_create_kv4(rt: *mut ab_runtime, cfg: *const ab_llama_config, comm: *mut ab_comm, out: *mut *mut ab_llama) -> c_int;
+    pub fn ab_llama_kv4cache(m: *mut ab_llama, out: *mut *mut ab_kv4cache) -> c_int;
     pub fn ab_llama_init_synthetic(m: *mut ab_llama, seed: u64, std: f32) -> c_int;
     pub fn ab_llama_weight(m: *mut ab_llama, which: i32, layer: u32, out_: *mut ab_tensor) -> c_int;
     pub fn ab_llama_cache(m: *mut ab_llama, out_: *mut *mut ab_kvcache) -> c_int;
