@@ -354,6 +354,16 @@ __global__ void __launch_bounds__(kThreads, kResident)
     constexpr uint32_t ROW = 16 * W;  // bytes of a row of codes
     constexpr uint32_t PART = S * (HP + 2);
     constexpr uint32_t M0 = 0x000f000fu, M1 = 0x00f000f0u;
+    // Columns of the weights. For f32 outputs a slot has two, the whole number and the rest. For
+    // bf16 outputs it has one, the weight rounded to fp16 (2^-12 of it, an eighth of the output's
+    // own rounding), and two sets of four slots share one operand.
+    constexpr bool F32 = sizeof(OT) == 4;
+    constexpr int NA = F32 ? NT : 1;
+    // Sums of bf16 outputs stay in the unit's accumulators. Those of f32 outputs start from zero
+    // every turn and are added to running ones, the rest's with the whole numbers', outside: the
+    // unit's own addition cuts off, and over a chain of positive terms that shows (5e-6 over 9
+    // turns, 1.4e-5 over 28).
+    constexpr bool KEEP = !F32;
     using St = Stage<W>;
     constexpr uint32_t RING = kStages * St::BYTES;  // a warp's turns
     constexpr uint32_t QF = NT * W * 2 * 32;        // operand words (uint2) of a unit's queries
@@ -604,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, kResident)
         // Weights are w = 2^(score - M). M is the largest score + log2 step of V so far, less 9,
         // moved when a w x step reaches 2^11: as for the queries, its whole number is one operand
         // column, exact in the sums, and the rest the other.
-        float o[NT][2 * W][2], l[NT], pm[NT], M[NT], cap[NT];
+        float o[NT][2 * W][2], kept[NA][2 * W][4], l[NT], pm[NT], M[NT], cap[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
             l[nt] = pm[nt] = M[nt] = 0.0f;
@@ -612,6 +622,11 @@ __global__ void __launch_bounds__(kThreads, kResident)
 #pragma unroll
             for (int i = 0; i < 2 * W; i++) o[nt][i][0] = o[nt][i][1] = 0.0f;
         }
+#pragma unroll
+        for (int n = 0; n < NA; n++)
+#pragma unroll
+            for (int i = 0; i < 2 * W; i++)
+                kept[n][i][0] = kept[n][i][1] = kept[n][i][2] = kept[n][i][3] = 0.0f;
         // Position 8 i + r of the 32, i = 0 .. 3, is lane r's: row r (even i) or 8 + r of the
         // operand of K's mma i / 2; V's takes the rows in the same order.
         const uint32_t k_at = W == 4   ? St::place(r, c)
@@ -663,8 +678,8 @@ __global__ void __launch_bounds__(kThreads, kResident)
                     for (int i = 0; i < 4; i++) {
                         const float step = bf16lo(ks[i]), sq = step * qscale[nt];
                         float x = fmaf(acc[i / 2][nt][2 * (i % 2)], sq, -M[nt]);
-                        x = fmaf(acc[i / 2][nt][2 * (i % 2) + 1], sq, x);
                         x = fmaf(fmaf(8.0f, step, bf16hi(ks[i])), qsum[nt], x);
+                        x = fmaf(acc[i / 2][nt][2 * (i % 2) + 1], sq, x);
                         const bool out = masked.value && (int32_t)(t + 8 * i + r) > limit[nt];
                         sc[nt][i] = out ? -INFINITY : x;
                         w[nt][i] = ex2(sc[nt][i]);
@@ -697,8 +712,13 @@ __global__ void __launch_bounds__(kThreads, kResident)
                             pm[nt] *= a;
 #pragma unroll
                             for (int i = 0; i < 2 * W; i++) {
-                                o[nt][i][0] *= a;
-                                o[nt][i][1] *= a;
+                                if constexpr (F32) {
+                                    o[nt][i][0] *= a;
+                                    o[nt][i][1] *= a;
+                                } else {
+                                    kept[0][i][nt] *= a;
+                                    kept[0][i][2 + nt] *= a;
+                                }
                             }
                         }
                         cap[nt] = 2048.0f;
@@ -706,23 +726,26 @@ __global__ void __launch_bounds__(kThreads, kResident)
                 }
                 weigh(std::true_type());
             }
-            uint32_t pb[NT][4];
+            uint32_t pb[NA][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
+            for (int i = 0; i < 4; i++) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
+                for (int nt = 0; nt < NT; nt++) {
                     l[nt] += w[nt][i];
                     if (!masked || (int32_t)(t + 8 * i + r) <= limit[nt])
                         pm[nt] = fmaf(w[nt][i], bf16hi(vs[i]), pm[nt]);
-                    // the nearest whole number, by way of 1.5 2^23
-                    const float first = (ws[nt][i] + 12582912.0f) - 12582912.0f;
-                    const __half2 two = __floats2half2_rn(first, ws[nt][i] - first);
-                    pb[nt][i] = transpose8(*reinterpret_cast<const uint32_t*>(&two));
+                    if constexpr (F32) {
+                        // the nearest whole number, by way of 1.5 2^23
+                        const float first = (ws[nt][i] + 12582912.0f) - 12582912.0f;
+                        const __half2 two = __floats2half2_rn(first, ws[nt][i] - first);
+                        pb[nt][i] = transpose8(*reinterpret_cast<const uint32_t*>(&two));
+                    }
+                }
+                if constexpr (!F32) {
+                    const __half2 two = __floats2half2_rn(ws[0][i], NT == 2 ? ws[NT - 1][i] : 0.0f);
+                    pb[0][i] = transpose8(*reinterpret_cast<const uint32_t*>(&two));
                 }
             }
-            // Sums of 32 positions start from zero and are added to the running ones, the rest's
-            // with the whole numbers', here: the unit's own addition cuts off, and over a long
-            // chain of positive terms that shows (1.4e-5 at 128k positions).
 #pragma unroll
             for (uint32_t k = 0; k < W; k++) {
                 uint32_t y[4];
@@ -734,14 +757,22 @@ __global__ void __launch_bounds__(kThreads, kResident)
                         for (int i = 0; i < 4; i++) y[i] >>= 8;
                     }
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        float a[4];
-                        mma16816_zero(a, y[0] & M0, y[0] & M1, y[1] & M0, y[1] & M1, pb[nt][0],
-                                      pb[nt][1]);
-                        mma16816(a, y[2] & M0, y[2] & M1, y[3] & M0, y[3] & M1, pb[nt][2],
-                                 pb[nt][3]);
-                        o[nt][2 * k + b][0] += a[0] + a[1];
-                        o[nt][2 * k + b][1] += a[2] + a[3];
+                    for (int n = 0; n < NA; n++) {
+                        if constexpr (KEEP) {
+                            float (&a)[4] = kept[n][2 * k + b];
+                            mma16816(a, y[0] & M0, y[0] & M1, y[1] & M0, y[1] & M1, pb[n][0],
+                                     pb[n][1]);
+                            mma16816(a, y[2] & M0, y[2] & M1, y[3] & M0, y[3] & M1, pb[n][2],
+                                     pb[n][3]);
+                        } else {
+                            float a[4];
+                            mma16816_zero(a, y[0] & M0, y[0] & M1, y[1] & M0, y[1] & M1, pb[n][0],
+                                          pb[n][1]);
+                            mma16816(a, y[2] & M0, y[2] & M1, y[3] & M0, y[3] & M1, pb[n][2],
+                                     pb[n][3]);
+                            o[n][2 * k + b][0] += a[0] + a[1];
+                            o[n][2 * k + b][1] += a[2] + a[3];
+                        }
                     }
                 }
             }
@@ -750,6 +781,16 @@ __global__ void __launch_bounds__(kThreads, kResident)
             stage = (stage + 1) % kStages;
         }
 
+        if constexpr (KEEP) {
+            // rows r and 8 + r of columns 2 c (slot c) and 2 c + 1 (slot c + 4)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int i = 0; i < 2 * W; i++) {
+                    o[nt][i][0] = kept[0][i][nt];
+                    o[nt][i][1] = kept[0][i][2 + nt];
+                }
+        }
         if (more) {
             open(after);
             set_queries(s_q + (nth + 1) % 2 * QF, s_slot[(nth + 1) % 2]);
