@@ -24,7 +24,8 @@
 // positions of one kv head) form one line that the blocks of one wave share equally, so rows of
 // unlike lengths and few rows of great length fill the device alike. A unit that several blocks
 // meet is joined by the last of them to finish, in line order: results do not depend on which
-// that is.
+// that is. Where units are more than blocks, each counts kLead tiles more than it has, about what
+// starting and joining it takes (counted by tiles alone, blocks of short units finished last).
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -47,6 +48,10 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kResident = 2;
 constexpr uint32_t kTurn = 32;              // positions of one warp's turn
 constexpr uint32_t kTile = kWarps * kTurn;  // positions of one block's turn
+// Tiles that a unit is taken to cost beyond its own: 0, 1, 2, 3 and 8 measured 69.5, 59.1, 56.4,
+// 57.7 and 62.5 us at 64 ragged rows of up to 8192 positions (32 heads of 8 kv heads, head 128,
+// bf16), 63.8, 54.7, 54.6, 54.1 and 57.1 at 256 of up to 1024 (12 heads, head 64, f32).
+constexpr uint32_t kLead = 2;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Kv4AttnParams {
@@ -57,6 +62,7 @@ struct Kv4AttnParams {
     uint32_t items;     // rows with a cache each, or blocks of query slots over one cache
     uint32_t per_item;  // kv heads x slot blocks of a row's group
     int shared;         // rows share one cache
+    uint32_t lead;      // tiles that a unit counts more than it has
     int qvec, ovec;     // 16-byte loads of q, four outputs at once
     float* part;        // [2 grid][slots][32 W + 2] partial results
     uint32_t* tickets;  // [items * per_item], zero between launches
@@ -391,11 +397,11 @@ __global__ void __launch_bounds__(kThreads, kResident)
     }
     uint32_t total = 0;  // tiles in all
     if (p.items == 1) {
-        if (warp == 0) total = tiles_of(item_length<S>(p, 0)) * p.per_item;
+        if (warp == 0) total = (tiles_of(item_length<S>(p, 0)) + p.lead) * p.per_item;
     } else {
         uint32_t sum = 0;
         for (uint32_t i = tid; i < p.items; i += kThreads)
-            sum += tiles_of(item_length<S>(p, i));
+            sum += tiles_of(item_length<S>(p, i)) + p.lead;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) s_scan[warp] = sum;
@@ -422,7 +428,8 @@ __global__ void __launch_bounds__(kThreads, kResident)
         uint32_t base = 0;
         for (uint32_t i0 = 0; i0 < p.items; i0 += kThreads) {
             const uint32_t i = i0 + tid;
-            const uint32_t n = i < p.items ? tiles_of(item_length<S>(p, i)) * p.per_item : 0;
+            const uint32_t n =
+                i < p.items ? (tiles_of(item_length<S>(p, i)) + p.lead) * p.per_item : 0;
             uint32_t upto = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -459,23 +466,23 @@ __global__ void __launch_bounds__(kThreads, kResident)
         n_tiles = tiles_of(len);
     }
     auto plan = [&](uint32_t at, Span& span) {  // the unit at `at`: the first warp's work
-        while (at - item_at >= n_tiles * p.per_item) {
-            item_at += n_tiles * p.per_item;
+        while (at - item_at >= (n_tiles + p.lead) * p.per_item) {
+            item_at += (n_tiles + p.lead) * p.per_item;
             item++;
             len = len1;
             len1 = item + 1 < p.items ? item_length<S>(p, item + 1) : 0;
             n_tiles = tiles_of(len);
         }
-        const uint32_t nth = (at - item_at) / n_tiles;
+        const uint32_t nth = (at - item_at) / (n_tiles + p.lead);
         if (lane == 0) {
             span.item = item;
             span.nth = nth;
             span.sub = nth / p.c.kv_heads;
             span.kvh = nth - span.sub * p.c.kv_heads;
-            span.at = item_at + nth * n_tiles;
+            span.at = item_at + nth * (n_tiles + p.lead) + p.lead;
             span.until = span.at + n_tiles;
-            span.t_begin = (at - span.at) * kTile;
-            span.t_end = min((min(end, span.until) - span.at) * kTile, len);
+            span.t_begin = (max(at, span.at) - span.at) * kTile;
+            span.t_end = min((min(end, span.until) - min(end, span.at)) * kTile, len);
         }
     };
     const unsigned char *ksrc, *vsrc;
@@ -583,6 +590,7 @@ __global__ void __launch_bounds__(kThreads, kResident)
 
     if (warp == 0) plan(begin, s_span[0]);
     __syncthreads();
+    if (s_span[0].at >= end) return;  // of its lead alone
     open(s_span[0]);
     read_queries(s_span[0]);
     set_queries(s_q, s_slot[0]);
@@ -590,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, kResident)
         const Span& span = s_span[nth % 3];
         Span& after = s_span[(nth + 1) % 3];
         const uint32_t next_at = min(end, span.until);
-        const bool more = next_at < end;
+        const bool more = next_at + p.lead < end;
         if (more && warp == 0) plan(next_at, after);
         __syncthreads();  // this unit's queries, the next one's place; the last one's outputs are read
         if (more) read_queries(after);
@@ -906,12 +914,14 @@ void record_one(ab_scheme* s, const char* label, Kv4AttnParams p) {
     auto* kernel = kv4_attention_kernel<W, NT, OT>;
     const uint64_t units = (uint64_t)p.items * p.per_item;
     const uint64_t tiles = units * ((p.c.seq + kTile - 1) / kTile);
-    if (tiles >> 31) invalid("kv4_attention: too much work for one call");
+    if ((tiles + kLead * units) >> 31) invalid("kv4_attention: too much work for one call");
     s->rt->activate();
     cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
                "kv4_attention shared memory");
     const uint32_t grid =
         (uint32_t)std::min<uint64_t>((uint64_t)s->rt->sm_count * kResident, tiles);
+    // with fewer units than blocks a stretch holds one or two: no difference, or 1 us lost
+    p.lead = units > grid ? kLead : 0;
     take_scratch(s, (uint64_t)grid * 2 * PART * 4, units, &p);
     s->add(label, [=](cudaStream_t stream) {
         return launch(stream, dim3(grid), dim3(kThreads), smem, true, kernel, p);
