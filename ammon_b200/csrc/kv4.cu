@@ -464,6 +464,8 @@ Kv4Rows rows_of(const ab_tensor& key, const ab_tensor& value, int rank_lo, int r
     r.kv_heads = key.dims[key.rank - 2];
     const uint64_t rows = numel(key) / ((uint64_t)r.head * r.kv_heads);
     if ((rows * r.kv_heads) >> 31) invalid("parameter `key`: too many vectors for one call");
+    if (((uintptr_t)key.data | (uintptr_t)value.data) % dtype_size(key.dtype))
+        invalid("parameter `key` / `value`: not aligned to its elements");
     r.rows = (uint32_t)rows;
     r.vectors = r.rows * r.kv_heads;
     r.vec = r.head % 8 == 0 && ((uintptr_t)key.data | (uintptr_t)value.data) % 16 == 0;
@@ -589,6 +591,8 @@ int ab_kv4cache_create(ab_runtime* rt, uint32_t layers, uint32_t seq_len, uint32
             fail(AB_ERR_ARGUMENT, "Kv4Cache dims must be non-zero");
         if (head_size > kKv4MaxHead)
             fail(AB_ERR_ARGUMENT, "Kv4Cache head size must be at most 128");
+        if ((double)layers * seq_len * kv_heads * batch > (double)(1ull << 40))
+            fail(AB_ERR_ARGUMENT, "Kv4Cache dims must make at most 2^40 vectors");
         auto* c = new ab_kv4cache{rt, layers, batch, seq_len, kv_heads, head_size, {}};
         try {
             rt->activate();

@@ -125,3 +125,21 @@ def test_cache_handle_refusals():
     assert _abi.lib().ab_kv4cache_layer(None, 0, None) == _abi.AB_ERR_ARGUMENT
     assert _abi.lib().ab_kv4cache_zero(None) == _abi.AB_ERR_ARGUMENT
     assert _abi.lib().ab_kv4cache_destroy(None) == _abi.AB_OK
+
+
+def test_rows_not_aligned_to_their_elements_are_refused(scheme):
+    for dtype, off in ((ab.F32, 2), (ab.BF16, 1)):
+        good, bad = fake((3, 2, 64), dtype), fake((3, 2, 64), dtype, FAKE + off)
+        for key, value in ((bad, good), (good, bad)):
+            refused(scheme, lambda: K.Kv4StoreKernel.prepare(None).record(
+                scheme, "s", key, value, layer(), step(3)), "not aligned")
+            refused(scheme, lambda: K.Kv4LoadKernel.prepare(None).record(
+                scheme, "l", layer(), step(), key, value), "not aligned")
+
+
+def test_more_vectors_than_a_call_takes_are_refused(scheme):
+    many = fake((1 << 28, 8, 16))
+    refused(scheme, lambda: K.Kv4StoreKernel.prepare(None).record(
+        scheme, "s", many, many, layer(kv=8, words=4), step(1 << 28)), "too many vectors")
+    refused(scheme, lambda: K.Kv4LoadKernel.prepare(None).record(
+        scheme, "l", layer(kv=8, seq=1 << 28, words=4), step(), many, many), "too many vectors")
