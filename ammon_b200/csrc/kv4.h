@@ -31,5 +31,26 @@ void record_kv4_store(ab_scheme* s, const char* label, ab_tensor key, ab_tensor 
 void record_kv4_attention(ab_scheme* s, const char* label, const float* q, uint32_t rows,
                           uint32_t heads, const Kv4View& cache, void* out, int32_t out_dtype,
                           const Step* step);
+// The same for rows of one shared cache and bf16 outputs on tcgen05 (kv4_prompt_tc.cu); false
+// when the call is not one it takes.
+bool record_kv4_prompt_tc(ab_scheme* s, const char* label, const float* q, uint32_t rows,
+                          uint32_t heads, const Kv4View& cache, void* out, const Step* step);
+// The scheme's scratch for parts and tickets (zero between launches). Its nodes run one after
+// the other, so they share it; a node that needs more makes it anew for itself and later ones.
+void kv4_take_scratch(ab_scheme* s, uint64_t part_bytes, uint64_t tickets, float** part,
+                      uint32_t** ticket);
+
+#ifdef __CUDACC__
+// One arrival at a ticket: what the block wrote before its last barrier is published with it,
+// what the earlier arrivals published is seen after it.
+__device__ __forceinline__ uint32_t kv4_arrive(uint32_t* ticket) {
+    uint32_t before;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;"
+                 : "=r"(before)
+                 : "l"(ticket)
+                 : "memory");
+    return before;
+}
+#endif
 
 }  // namespace ab

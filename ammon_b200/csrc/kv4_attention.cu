@@ -52,6 +52,8 @@ constexpr uint32_t kTile = kWarps * kTurn;  // positions of one block's turn
 // 57.7 and 62.5 us at 64 ragged rows of up to 8192 positions (32 heads of 8 kv heads, head 128,
 // bf16), 63.8, 54.7, 54.6, 54.1 and 57.1 at 256 of up to 1024 (12 heads, head 64, f32).
 constexpr uint32_t kLead = 2;
+// Query slots of one kv head over one cache from which on tcgen05 takes them (bf16 outputs).
+constexpr uint64_t kTensorSlots = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Kv4AttnParams {
@@ -179,17 +181,6 @@ __device__ __forceinline__ void load_v(uint32_t at, uint32_t (&y)[4]) {
                  : "=r"(y[0]), "=r"(y[1]), "=r"(y[2]), "=r"(y[3])
                  : "r"(at)
                  : "memory");
-}
-
-// One arrival at a ticket: what the block wrote before its last barrier is published with it,
-// what the earlier arrivals published is seen after it.
-__device__ __forceinline__ uint32_t arrive(uint32_t* ticket) {
-    uint32_t before;
-    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;"
-                 : "=r"(before)
-                 : "l"(ticket)
-                 : "memory");
-    return before;
 }
 
 // Positions that the rows of item i attend over.
@@ -865,7 +856,7 @@ __global__ void __launch_bounds__(kThreads, kResident)
                 const uint32_t first = line.block_of(span.at);
                 const uint32_t parts = line.block_of(span.until - 1) - first + 1;
                 uint32_t* ticket = p.tickets + (uint64_t)unit.item * p.per_item + span.nth;
-                if (arrive(ticket) == parts - 1) {
+                if (kv4_arrive(ticket) == parts - 1) {
                     *ticket = 0;
                     s_job[jobs++] = Job{unit.item, unit.kvh, unit.sub, first, parts};
                 }
@@ -881,29 +872,6 @@ __global__ void __launch_bounds__(kThreads, kResident)
                          tid, so, s_m, s_l);
         __syncthreads();
     }
-}
-
-// The scheme's scratch for parts and tickets (zero between launches). Its nodes run one after
-// the other, so they share it; a node that needs more makes it anew for itself and later ones.
-void take_scratch(ab_scheme* s, uint64_t part_bytes, uint64_t tickets, Kv4AttnParams* p) {
-    auto& have = s->kv4;
-    if (have.part_bytes < part_bytes) {
-        void* d = nullptr;
-        cuda_check(cudaMalloc(&d, part_bytes), "cudaMalloc");
-        s->owned.push_back(d);
-        have.part = d;
-        have.part_bytes = part_bytes;
-    }
-    if (have.tickets_n < tickets) {
-        void* d = nullptr;
-        cuda_check(cudaMalloc(&d, tickets * 4), "cudaMalloc");
-        s->owned.push_back(d);
-        cuda_check(clear_device(s->rt, d, tickets * 4), "clear tickets");
-        have.tickets = (uint32_t*)d;
-        have.tickets_n = tickets;
-    }
-    p->part = (float*)have.part;
-    p->tickets = have.tickets;
 }
 
 template <int W, int NT, typename OT>
@@ -922,7 +890,7 @@ void record_one(ab_scheme* s, const char* label, Kv4AttnParams p) {
         (uint32_t)std::min<uint64_t>((uint64_t)s->rt->sm_count * kResident, tiles);
     // with fewer units than blocks a stretch holds one or two: no difference, or 1 us lost
     p.lead = units > grid ? kLead : 0;
-    take_scratch(s, (uint64_t)grid * 2 * PART * 4, units, &p);
+    kv4_take_scratch(s, (uint64_t)grid * 2 * PART * 4, units, &p.part, &p.tickets);
     s->add(label, [=](cudaStream_t stream) {
         return launch(stream, dim3(grid), dim3(kThreads), smem, true, kernel, p);
     });
@@ -946,6 +914,28 @@ void record_width(ab_scheme* s, const char* label, Kv4AttnParams p, int32_t out_
 
 }  // namespace
 
+void kv4_take_scratch(ab_scheme* s, uint64_t part_bytes, uint64_t tickets, float** part,
+                      uint32_t** ticket) {
+    auto& have = s->kv4;
+    if (have.part_bytes < part_bytes) {
+        void* d = nullptr;
+        cuda_check(cudaMalloc(&d, part_bytes), "cudaMalloc");
+        s->owned.push_back(d);
+        have.part = d;
+        have.part_bytes = part_bytes;
+    }
+    if (have.tickets_n < tickets) {
+        void* d = nullptr;
+        cuda_check(cudaMalloc(&d, tickets * 4), "cudaMalloc");
+        s->owned.push_back(d);
+        cuda_check(clear_device(s->rt, d, tickets * 4), "clear tickets");
+        have.tickets = (uint32_t*)d;
+        have.tickets_n = tickets;
+    }
+    *part = (float*)have.part;
+    *ticket = have.tickets;
+}
+
 void record_kv4_attention(ab_scheme* s, const char* label, const float* q, uint32_t rows,
                           uint32_t heads, const Kv4View& cache, void* out, int32_t out_dtype,
                           const Step* step) {
@@ -957,6 +947,10 @@ void record_kv4_attention(ab_scheme* s, const char* label, const float* q, uint3
     if (!s->rt)
         fail(AB_ERR_ARGUMENT, "kv4_attention: the scheme needs a runtime (it allocates the split "
                               "scratch)");
+    const uint64_t slots = (uint64_t)rows * (heads / cache.kv_heads);  // over one shared cache
+    if (cache.row_stride == 0 && out_dtype == AB_BF16 && slots >= kTensorSlots &&
+        record_kv4_prompt_tc(s, label, q, rows, heads, cache, out, step))
+        return;
     Kv4AttnParams p = {};
     p.c = cache;
     p.q = q;
