@@ -7,11 +7,13 @@
 // and m' enter per position, outside the products.
 //
 // One block takes 128 slots of a kv head over a run of 64-position tiles, a slot a TMEM lane:
-//  - warps 8-11 read a tile's codes (the next tile's are on their way meanwhile), write them as
+//  - warps 16-19 read a tile's codes (the next tile's are on their way meanwhile), write them as
 //    bf16 operands of K and V in the 128-byte-swizzled layout, and the tile's steps and offsets;
-//  - warp 12 (one thread) issues tcgen05.mma: S = Q.(K codes)^T into one of two 64-column TMEM
-//    buffers, a tile ahead, and O += P.(V codes), V being an MN-major operand of the same layout;
-//  - warps 0-7, two threads a slot, make scores of S, keep the slot's maximum and sums, write
+//  - warp 20 (one thread) issues tcgen05.mma: S = Q.(K codes)^T into one of two 64-column TMEM
+//    buffers, a tile ahead, and O += P.(V codes), V being an MN-major operand of the same layout.
+//    Q and P are operands in TMEM: from shared memory, each product read 4 KB of them beside the
+//    2 or 4 KB of codes, which made shared memory the bound;
+//  - warps 0-15, four threads a slot, make scores of S, keep the slot's maximum and sums, write
 //    P = p s of V as the next A operand, and rescale O when the maximum grew by more than
 //    kRescale since the scale that O is kept in.
 // Q and P are bf16 pairs, value and rest (two products each): 16 bits, 2^-18 of a query or a
@@ -39,12 +41,15 @@ namespace {
 
 constexpr uint32_t kRows = 128;      // slots of a block (TMEM lanes)
 constexpr uint32_t kTile = 64;       // positions
-constexpr uint32_t kStages = 3;      // tiles unpacked at a time
-constexpr uint32_t kSoftmax = 256;   // threads of warps 0-7
-constexpr uint32_t kUnpack = 128;    // of warps 8-11
+constexpr uint32_t kStages = 4;      // tiles unpacked at a time
+constexpr uint32_t kShare = 4;       // threads of a slot
+constexpr uint32_t kCols = kTile / kShare;
+constexpr uint32_t kSoftmax = kRows * kShare;  // threads of warps 0-15
+constexpr uint32_t kUnpack = 128;              // of warps 16-19
+constexpr uint32_t kUnpackWarp = kSoftmax / 32, kMmaWarp = kUnpackWarp + kUnpack / 32;
 constexpr uint32_t kThreads = kSoftmax + kUnpack + 32;
-constexpr uint32_t kTmemCols = 256;  // S at columns 0 and 64, O from 128
-constexpr uint32_t kTmemO = 128;
+// Columns of TMEM: S twice, O, Q (value, rest), P (value, rest) twice.
+constexpr uint32_t kTmemCols = 512, kTmemO = 128, kTmemQ = 256, kTmemP = 384;
 constexpr uint32_t kMinTiles = 4;    // a part has at least so many
 constexpr float kRescale = 11.5f;    // base 2: P stays below 2^kRescale steps of V
 constexpr float kLog2e = 1.4426950408889634f;
@@ -63,14 +68,11 @@ struct PromptParams {
 
 template <int HD>
 struct Layout {
-    static constexpr uint32_t Q = kRows * HD * 2;     // value, then rest
-    static constexpr uint32_t P = kRows * kTile * 2;  // value, then rest
-    static constexpr uint32_t T = kTile * HD * 2;     // K or V of a tile
-    static constexpr uint32_t P_AT = 2 * Q, KV_AT = P_AT + 2 * P;
-    static constexpr uint32_t SCALES_AT = KV_AT + kStages * 2 * T;  // [stage][K, V][64] (s, m')
-    static constexpr uint32_t RED_AT = SCALES_AT + kStages * 2 * kTile * 8;
-    // maxima [2 tiles][2 halves][128]; sums of q, of weights, of weights x m' [2 halves][128]
-    static constexpr uint32_t BYTES = RED_AT + 10 * kRows * 4;
+    static constexpr uint32_t T = kTile * HD * 2;  // K or V of a tile
+    static constexpr uint32_t SCALES_AT = kStages * 2 * T;  // [stage][K, V][s, m'][64]
+    static constexpr uint32_t RED_AT = SCALES_AT + kStages * 4 * kTile * 4;
+    // maxima [2 tiles][kShare][128]; sums of q, of weights, of weights x m' [kShare][128]
+    static constexpr uint32_t BYTES = RED_AT + 5 * kShare * kRows * 4;
 };
 
 // Byte offset of 16-byte chunk c (0..7) of row r in a block of 128-byte rows with the 128-byte
@@ -88,11 +90,37 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// Two floats at a time.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "mov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
 // Two floats as a bf16 pair and the pair of what rounding left.
 __device__ __forceinline__ void split(float a, float b, uint32_t* value, uint32_t* rest) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     *value = *reinterpret_cast<const uint32_t*>(&h);
-    const __nv_bfloat162 l = __floats2bfloat162_rn(a - bf16lo(*value), b - bf16hi(*value));
+    const float2 left = add2(make_float2(a, b), make_float2(-bf16lo(*value), -bf16hi(*value)));
+    const __nv_bfloat162 l = __floats2bfloat162_rn(left.x, left.y);
     *rest = *reinterpret_cast<const uint32_t*>(&l);
 }
 // Codes of a word less 8, as bf16: elements 0 4 1 5 2 6 3 7. A code stands in the low bits of a
@@ -134,14 +162,14 @@ __device__ __forceinline__ void put_out(const PromptParams& p, uint64_t orow, ui
         }
     }
 }
-// Barrier of the 64 threads that share 32 slots, with the AND of a predicate over them.
-__device__ __forceinline__ bool pair_sync_and(uint32_t warp, bool v) {
+// Barrier of the threads that share 32 slots, with the AND of a predicate over them.
+__device__ __forceinline__ bool share_sync_and(uint32_t warp, bool v) {
     uint32_t r;
     asm volatile(
         "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\t"
-        "bar.red.and.pred p, %2, 64, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        "bar.red.and.pred p, %2, %3, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(r)
-        : "r"((uint32_t)v), "r"(1 + warp % 4)
+        : "r"((uint32_t)v), "r"(1 + warp % 4), "n"(32 * kShare)
         : "memory");
     return r != 0;
 }
@@ -152,8 +180,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     using LY = Layout<HD>;
     constexpr uint32_t BOX = HD / 64;  // 64-dim blocks of a row
     extern __shared__ __align__(16) unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t full[kStages], empty[kStages], s_full[2], s_free[2], p_full,
-        pv_done, done;
+    __shared__ __align__(8) uint64_t full[kStages], empty[kStages], s_full[2], s_free[2], p_full[2],
+        pv_done[2], done;
     __shared__ uint32_t s_tmem, s_most[4];
     __shared__ int s_fail, s_last;
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -163,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t kvh = blockIdx.y, slot = blockIdx.x * kRows + tid % kRows;
 
     pdl_wait();
-    // the slot's row, head and last position; both threads of a slot need them
+    // the slot's row, head and last position; each of its threads needs them
     const uint32_t row = slot / p.group;
     const bool live = tid < kSoftmax && row < p.rows;
     int32_t limit = -1;
@@ -195,111 +223,132 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (uint32_t i = 0; i < 2; i++) {
             mbar_init(smem_u32(&s_full[i]), 1);
             mbar_init(smem_u32(&s_free[i]), kSoftmax);
+            mbar_init(smem_u32(&p_full[i]), kSoftmax);
+            mbar_init(smem_u32(&pv_done[i]), 1);
         }
-        mbar_init(smem_u32(&p_full), kSoftmax);
-        mbar_init(smem_u32(&pv_done), 1);
         mbar_init(smem_u32(&done), 1);
         fence_barrier_init();
         s_fail = 0;
     }
     if (warp == 0) tmem_alloc(smem_u32(&s_tmem), kTmemCols);
-    if (tid < kSoftmax) {
-        // the slot's queries times log2(e) / sqrt(head): this half's dims
-        const uint32_t r = tid % kRows, half = tid / kRows;
-        const float by = kLog2e / sqrtf((float)p.c.head);
-        const float* q = p.q + orow * p.c.head;
-        float sum = 0.0f;
-#pragma unroll
-        for (uint32_t j = 0; j < HD / 16; j++) {
-            const uint32_t chunk = half * (HD / 16) + j, d = chunk * 8;
-            float v[8];
-#pragma unroll
-            for (uint32_t k = 0; k < 8; k += 4) {
-                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (limit >= 0 && d + k < p.c.head) {
-                    if (p.qvec) {
-                        x = *reinterpret_cast<const float4*>(q + d + k);
-                    } else {
-                        const uint32_t left = p.c.head - d - k;
-                        x.x = q[d + k];
-                        if (left > 1) x.y = q[d + k + 1];
-                        if (left > 2) x.z = q[d + k + 2];
-                        if (left > 3) x.w = q[d + k + 3];
-                    }
-                }
-                v[k] = x.x * by;
-                v[k + 1] = x.y * by;
-                v[k + 2] = x.z * by;
-                v[k + 3] = x.w * by;
-                sum += (v[k] + v[k + 1]) + (v[k + 2] + v[k + 3]);
-            }
-            uint32_t value[4], rest[4];
-#pragma unroll
-            for (int k = 0; k < 4; k++) split(v[k], v[k + 4], &value[k], &rest[k]);
-            const uint32_t at = base + chunk / 8 * (kRows * 128) + row_chunk(r, chunk % 8);
-            put(at, value);
-            put(at + LY::Q, rest);
-        }
-        red[(4 + half) * kRows + r] = sum;
-        fence_proxy_async_smem();
-    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
+    const uint32_t mine = tmem + ((warp % 4 * 32) << 16);  // this warp's lanes
+    const uint32_t r = tid % kRows, nth = tid / kRows;      // of the threads of slots
+    if (tid < kSoftmax) {
+        // the slot's queries times log2(e) / sqrt(head): this thread's dims
+        const float by = kLog2e / sqrtf((float)p.c.head);
+        const float* q = p.q + orow * p.c.head;
+        float sum = 0.0f;
+#pragma unroll
+        for (uint32_t j = 0; j < HD / (16 * kShare); j++) {
+            uint32_t value[8], rest[8];
+#pragma unroll
+            for (uint32_t e = 0; e < 2; e++) {
+                const uint32_t d = nth * (HD / kShare) + 16 * j + 8 * e;
+                float v[8];
+#pragma unroll
+                for (uint32_t k = 0; k < 8; k += 4) {
+                    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (limit >= 0 && d + k < p.c.head) {
+                        if (p.qvec) {
+                            x = *reinterpret_cast<const float4*>(q + d + k);
+                        } else {
+                            const uint32_t left = p.c.head - d - k;
+                            x.x = q[d + k];
+                            if (left > 1) x.y = q[d + k + 1];
+                            if (left > 2) x.z = q[d + k + 2];
+                            if (left > 3) x.w = q[d + k + 3];
+                        }
+                    }
+                    v[k] = x.x * by;
+                    v[k + 1] = x.y * by;
+                    v[k + 2] = x.z * by;
+                    v[k + 3] = x.w * by;
+                    sum += (v[k] + v[k + 1]) + (v[k + 2] + v[k + 3]);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    split(v[k], v[k + 4], &value[4 * e + k], &rest[4 * e + k]);
+            }
+            const uint32_t at = mine + kTmemQ + nth * (HD / (2 * kShare)) + 8 * j;
+            tmem_st8(at, value);
+            tmem_st8(at + HD / 2, rest);
+        }
+        red[(2 * kShare + nth) * kRows + r] = sum;
+        tmem_wait_st();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
 
     float m_ref = -INFINITY, l = 0.0f, pm = 0.0f;
-    if (warp >= 8 && warp < 12) {
+    if (warp >= kUnpackWarp && warp < kMmaWarp) {
         // ---- codes to operands: a thread half of a position's chunks (32 dims each) ----
-        const uint32_t u = tid - kSoftmax, r = u / 2, odd = u % 2;
+        const uint32_t u = tid - kSoftmax, line = u / 2, odd = u % 2;
         const uint64_t head0 = (uint64_t)kvh * p.c.seq;
         const uint32_t chunks = p.c.words / 4;
-        uint4 w[2][BOX];
-        uint32_t sc = 0;  // of K (even threads) or V
-        auto read = [&](uint32_t tile) {
-            const uint32_t pos = (t_lo + tile) * kTile + r;
+        struct Raw {
+            uint4 w[2][BOX];
+            uint32_t sc;  // of K (even threads) or V
+        };
+        auto read = [&](uint32_t tile, Raw& raw) {
+            const uint32_t pos = (t_lo + tile) * kTile + line;
             const bool in = tile < n && pos < until;
 #pragma unroll
             for (int x = 0; x < 2; x++)
 #pragma unroll
                 for (uint32_t b = 0; b < BOX; b++) {
                     const uint32_t c = 2 * b + odd;
-                    w[x][b] = make_uint4(0, 0, 0, 0);
+                    raw.w[x][b] = make_uint4(0, 0, 0, 0);
                     if (in && c < chunks)
-                        w[x][b] = ld16(p.c.codes[x] + (head0 + pos) * p.c.words + 4 * c);
+                        raw.w[x][b] = ld16(p.c.codes[x] + (head0 + pos) * p.c.words + 4 * c);
                 }
-            sc = 0;
-            if (in) sc = __ldcg(p.c.scales[odd] + head0 + pos);
+            raw.sc = 0;
+            if (in) raw.sc = __ldcg(p.c.scales[odd] + head0 + pos);
         };
-        read(0);
-        for (uint32_t i = 0; i < n; i++) {
+        auto write = [&](uint32_t i, const Raw& raw) {
             const uint32_t s = i % kStages;
             if (i >= kStages && !mbar_wait_bounded(smem_u32(&empty[s]), (i / kStages - 1) & 1,
-                                                   p.flags)) {
-                s_fail = 1;
-                break;
-            }
-            const uint32_t to = base + LY::KV_AT + s * 2 * LY::T;
+                                                   p.flags))
+                return false;
+            const uint32_t to = base + s * 2 * LY::T;
 #pragma unroll
             for (int x = 0; x < 2; x++)
 #pragma unroll
                 for (uint32_t b = 0; b < BOX; b++) {
-                    const uint32_t word[4] = {w[x][b].x, w[x][b].y, w[x][b].z, w[x][b].w};
+                    const uint4& w = raw.w[x][b];
+                    const uint32_t word[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                     for (uint32_t k = 0; k < 4; k++) {
                         uint32_t v[4];
                         unpack(word[k], v);
-                        put(to + x * LY::T + b * (kTile * 128) + row_chunk(r, 4 * odd + k), v);
+                        put(to + x * LY::T + b * (kTile * 128) + row_chunk(line, 4 * odd + k), v);
                     }
                 }
-            float2* scales = reinterpret_cast<float2*>(smem + LY::SCALES_AT) +
-                             (s * 2 + odd) * kTile + r;
-            *scales = make_float2(bf16lo(sc), fmaf(8.0f, bf16lo(sc), bf16hi(sc)));
+            float* scales =
+                reinterpret_cast<float*>(smem + LY::SCALES_AT) + (s * 2 + odd) * (2 * kTile) + line;
+            scales[0] = bf16lo(raw.sc);
+            scales[kTile] = fmaf(8.0f, bf16lo(raw.sc), bf16hi(raw.sc));
             fence_proxy_async_smem();
             mbar_arrive(smem_u32(&full[s]));
-            read(i + 1);
+            return true;
+        };
+        // two tiles are on their way
+        Raw even, uneven;
+        read(0, even);
+        read(1, uneven);
+        bool ok = true;
+        for (uint32_t i = 0; i < n && ok; i += 2) {
+            ok = write(i, even);
+            read(i + 2, even);
+            if (ok && i + 1 < n) ok = write(i + 1, uneven);
+            read(i + 3, uneven);
         }
-    } else if (warp == 12) {
+        if (!ok) s_fail = 1;
+    } else if (warp == kMmaWarp) {
         if (lane == 0 && n > 0) {
             const uint32_t idesc_s = tc_idesc_bf16(kRows, kTile);
             const uint32_t idesc_o = tc_idesc_bf16(kRows, HD) | kIdescBMajorMN;
@@ -311,17 +360,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (i >= 2 && !mbar_wait_bounded(smem_u32(&s_free[i % 2]), (i / 2 - 1) & 1, p.flags))
                     return false;
                 tc_fence_after();
-                const uint32_t k_at = base + LY::KV_AT + s * 2 * LY::T;
+                const uint32_t k_at = base + s * 2 * LY::T;
                 const uint32_t d = tmem + (i % 2) * kTile;
 #pragma unroll
                 for (uint32_t b = 0; b < BOX; b++) {
-                    const uint64_t qv = sw128_desc(base + b * (kRows * 128));
-                    const uint64_t qr = sw128_desc(base + LY::Q + b * (kRows * 128));
                     const uint64_t kd = sw128_desc(k_at + b * (kTile * 128));
 #pragma unroll
                     for (uint32_t k = 0; k < 4; k++) {
-                        tc_mma_bf16(d, qv + 2 * k, kd + 2 * k, idesc_s, (b | k) != 0);
-                        tc_mma_bf16(d, qr + 2 * k, kd + 2 * k, idesc_s, 1);
+                        const uint32_t q = tmem + kTmemQ + 32 * b + 8 * k;
+                        tc_mma_bf16_ta(d, q, kd + 2 * k, idesc_s, (b | k) != 0);
+                        tc_mma_bf16_ta(d, q + HD / 2, kd + 2 * k, idesc_s, 1);
                     }
                 }
                 tc_commit(smem_u32(&s_full[i % 2]));
@@ -333,64 +381,80 @@ __global__ void __launch_bounds__(kThreads, 1)
                     ok = false;
                     break;
                 }
-                if (!mbar_wait_bounded(smem_u32(&p_full), i & 1, p.flags)) {
+                if (!mbar_wait_bounded(smem_u32(&p_full[i % 2]), (i / 2) & 1, p.flags)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                const uint32_t v_at = base + LY::KV_AT + (i % kStages * 2 + 1) * LY::T;
-                const uint64_t pv = sw128_desc(base + LY::P_AT);
-                const uint64_t pr = sw128_desc(base + LY::P_AT + LY::P);
+                const uint32_t v_at = base + (i % kStages * 2 + 1) * LY::T;
+                const uint32_t w = tmem + kTmemP + i % 2 * kTile;
 #pragma unroll
                 for (uint32_t k = 0; k < kTile / 16; k++) {
                     const uint64_t vd = sw128_desc_mn(v_at + k * 16 * 128, kTile * 128);
-                    tc_mma_bf16(tmem + kTmemO, pv + 2 * k, vd, idesc_o, (i | k) != 0);
-                    tc_mma_bf16(tmem + kTmemO, pr + 2 * k, vd, idesc_o, 1);
+                    tc_mma_bf16_ta(tmem + kTmemO, w + 8 * k, vd, idesc_o, (i | k) != 0);
+                    tc_mma_bf16_ta(tmem + kTmemO, w + kTile / 2 + 8 * k, vd, idesc_o, 1);
                 }
-                tc_commit(smem_u32(&pv_done));
+                tc_commit(smem_u32(&pv_done[i % 2]));
                 tc_commit(smem_u32(&empty[i % kStages]));
             }
             if (!ok) s_fail = 1;
         }
         if (lane == 0) tc_commit(smem_u32(&done));  // all that this thread issued
-    } else if (warp < 8) {
-        // ---- weights: thread `half` of a slot has columns 32 half .. of S, HD / 2 half .. of O --
-        const uint32_t r = tid % kRows, half = tid / kRows;
-        const uint32_t mine = tmem + ((warp % 4 * 32) << 16);  // this warp's lanes
-        const float qsum = red[4 * kRows + r] + red[5 * kRows + r];
+    } else if (tid < kSoftmax) {
+        // ---- weights: thread `nth` of a slot has columns kCols nth .. of S, HD / kShare nth .. of
+        // O ----
+        float qs = 0.0f;
+#pragma unroll
+        for (uint32_t k = 0; k < kShare; k++) qs += red[(2 * kShare + k) * kRows + r];
+        const float2 qsum = make_float2(qs, qs);
         bool ok = true, failed = false;
         for (uint32_t i = 0; i < n; i++) {
             bool w = mbar_wait_bounded(smem_u32(&s_full[i % 2]), (i / 2) & 1, p.flags);
             w = mbar_wait_bounded(smem_u32(&full[i % kStages]), (i / kStages) & 1, p.flags) && w;
+            // this P has been multiplied
+            if (i >= 2)
+                w = mbar_wait_bounded(smem_u32(&pv_done[i % 2]), (i / 2 - 1) & 1, p.flags) && w;
+            __syncwarp();
             tc_fence_after();
-            float x[32];
-            tmem_ld16(mine + (i % 2) * kTile + half * 32, x);
-            tmem_ld16(mine + (i % 2) * kTile + half * 32 + 16, x + 16);
+            float xs[kCols];
+            tmem_ld16(mine + (i % 2) * kTile + nth * kCols, xs);
             tc_fence_before();
             mbar_arrive(smem_u32(&s_free[i % 2]));
-            const float4* ks = reinterpret_cast<const float4*>(smem + LY::SCALES_AT) +
-                               i % kStages * kTile + half * 16;
-            const float4* vs = ks + kTile / 2;
+            const float4* scales = reinterpret_cast<const float4*>(smem + LY::SCALES_AT) +
+                                   i % kStages * kTile + nth * (kCols / 4);
+            float2 x[kCols / 2], vs[kCols / 2], vm[kCols / 2];
 #pragma unroll
-            for (int j = 0; j < 16; j++) {
-                const float4 k = ks[j];
-                x[2 * j] = fmaf(x[2 * j], k.x, qsum * k.y);
-                x[2 * j + 1] = fmaf(x[2 * j + 1], k.z, qsum * k.w);
+            for (uint32_t j = 0; j < kCols / 4; j++) {
+                const float4 ks = scales[j], km = scales[kTile / 4 + j];
+                const float4 s4 = scales[2 * (kTile / 4) + j], m4 = scales[3 * (kTile / 4) + j];
+                x[2 * j] = fma2(make_float2(xs[4 * j], xs[4 * j + 1]), make_float2(ks.x, ks.y),
+                                mul2(qsum, make_float2(km.x, km.y)));
+                x[2 * j + 1] = fma2(make_float2(xs[4 * j + 2], xs[4 * j + 3]),
+                                    make_float2(ks.z, ks.w),
+                                    mul2(qsum, make_float2(km.z, km.w)));
+                vs[2 * j] = make_float2(s4.x, s4.y);
+                vs[2 * j + 1] = make_float2(s4.z, s4.w);
+                vm[2 * j] = make_float2(m4.x, m4.y);
+                vm[2 * j + 1] = make_float2(m4.z, m4.w);
             }
-            const int32_t t0 = (int32_t)((t_lo + i) * kTile + half * 32);
-            const int32_t seen = limit - t0;  // columns 0 .. seen are attended over
-            if (seen < 31) {
+            // columns 0 .. seen are attended over; what the others hold is not used, NaN or not
+            const int32_t seen = limit - (int32_t)((t_lo + i) * kTile + nth * kCols);
+            if (seen < (int32_t)kCols - 1) {
 #pragma unroll
-                for (int j = 0; j < 32; j++)
-                    if (j > seen) x[j] = -INFINITY;
+                for (int j = 0; j < (int)kCols / 2; j++) {
+                    if (2 * j > seen) x[j].x = -INFINITY, vs[j].x = vm[j].x = 0.0f;
+                    if (2 * j + 1 > seen) x[j].y = -INFINITY, vs[j].y = vm[j].y = 0.0f;
+                }
             }
-            float most = x[0];
+            float most = fmaxf(x[0].x, x[0].y);
 #pragma unroll
-            for (int j = 1; j < 32; j++) most = fmaxf(most, x[j]);
-            red[((i & 1) * 2 + half) * kRows + r] = most;
-            ok = pair_sync_and(warp, w && !failed);
+            for (uint32_t j = 1; j < kCols / 2; j++) most = fmaxf(fmaxf(most, x[j].x), x[j].y);
+            float* maxima = red + (i & 1) * (kShare * kRows) + r;
+            maxima[nth * kRows] = most;
+            ok = share_sync_and(warp, w && !failed);
             if (!ok) break;
-            most = fmaxf(most, red[((i & 1) * 2 + (half ^ 1)) * kRows + r]);
+#pragma unroll
+            for (uint32_t k = 0; k < kShare; k++) most = fmaxf(most, maxima[k * kRows]);
             float alpha = 1.0f;
             bool rescale = false;
             if (most != -INFINITY && (m_ref == -INFINITY || most > m_ref + kRescale)) {
@@ -400,72 +464,64 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 m_ref = most;
             }
-            const float m0 = m_ref == -INFINITY ? 0.0f : m_ref;  // nothing seen: weights of 0
-            float sum = 0.0f, off = 0.0f;
+            const float m0 = m_ref == -INFINITY ? 0.0f : -m_ref;  // nothing seen: weights of 0
+            const float2 m2 = make_float2(m0, m0);
+            float2 sum = make_float2(0.0f, 0.0f), off = sum;
 #pragma unroll
-            for (int j = 0; j < 16; j++) {
-                const float4 v = vs[j];
-                const float a = ex2(x[2 * j] - m0), b = ex2(x[2 * j + 1] - m0);
-                sum += a + b;
-                x[2 * j] = a * v.x;
-                x[2 * j + 1] = b * v.z;
-                if (seen < 31) {  // what lies past the row's position is not used, NaN or not
-                    if (2 * j > seen) x[2 * j] = 0.0f;
-                    if (2 * j + 1 > seen) x[2 * j + 1] = 0.0f;
-                    off = fmaf(a, 2 * j > seen ? 0.0f : v.y, off);
-                    off = fmaf(b, 2 * j + 1 > seen ? 0.0f : v.w, off);
-                } else {
-                    off = fmaf(a, v.y, off);
-                    off = fmaf(b, v.w, off);
-                }
+            for (uint32_t j = 0; j < kCols / 2; j++) {
+                const float2 y = add2(x[j], m2);
+                const float2 a = make_float2(ex2(y.x), ex2(y.y));
+                sum = add2(sum, a);
+                off = fma2(a, vm[j], off);
+                x[j] = mul2(a, vs[j]);
             }
-            l = fmaf(l, alpha, sum);
-            pm = fmaf(pm, alpha, off);
-            // P's place and O are free once the tile before is in O
-            if (i >= 1 && !mbar_wait_bounded(smem_u32(&pv_done), (i - 1) & 1, p.flags))
-                failed = true;
-            tc_fence_after();
+            l = fmaf(l, alpha, sum.x + sum.y);
+            pm = fmaf(pm, alpha, off.x + off.y);
+            // O is at rest once the tile before is in it
             if (i >= 1 && __any_sync(0xffffffffu, rescale)) {
+                if (!mbar_wait_bounded(smem_u32(&pv_done[(i - 1) % 2]), ((i - 1) / 2) & 1, p.flags))
+                    failed = true;
+                __syncwarp();
+                tc_fence_after();
 #pragma unroll
-                for (uint32_t c = 0; c < HD / 32; c++) {
+                for (uint32_t c = 0; c < HD / (16 * kShare); c++) {
                     float o[16];
-                    const uint32_t at = mine + kTmemO + half * (HD / 2) + 16 * c;
+                    const uint32_t at = mine + kTmemO + nth * (HD / kShare) + 16 * c;
                     tmem_ld16(at, o);
 #pragma unroll
                     for (int k = 0; k < 16; k++) o[k] *= alpha;
                     tmem_st16(at, o);
                 }
-                tmem_wait_st();
             }
+            uint32_t value[8], rest[8];
 #pragma unroll
-            for (uint32_t c = 0; c < 4; c++) {
-                uint32_t value[4], rest[4];
-#pragma unroll
-                for (int k = 0; k < 4; k++)
-                    split(x[8 * c + 2 * k], x[8 * c + 2 * k + 1], &value[k], &rest[k]);
-                const uint32_t at = base + LY::P_AT + row_chunk(r, half * 4 + c);
-                put(at, value);
-                put(at + LY::P, rest);
-            }
-            fence_proxy_async_smem();
+            for (int k = 0; k < 8; k++) split(x[k].x, x[k].y, &value[k], &rest[k]);
+            const uint32_t at = mine + kTmemP + i % 2 * kTile + nth * (kCols / 2);
+            tmem_st8(at, value);
+            tmem_st8(at + kTile / 2, rest);
+            tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(smem_u32(&p_full));
+            mbar_arrive(smem_u32(&p_full[i % 2]));
         }
         bool w = true;
-        if (ok && n > 0) w = mbar_wait_bounded(smem_u32(&pv_done), (n - 1) & 1, p.flags);
-        red[(6 + half) * kRows + r] = l;
-        red[(8 + half) * kRows + r] = pm;
-        ok = pair_sync_and(warp, ok && w && !failed);
-        l = red[6 * kRows + r] + red[7 * kRows + r];
-        pm = red[8 * kRows + r] + red[9 * kRows + r];
+        if (ok && n > 0) w = mbar_wait_bounded(smem_u32(&pv_done[(n - 1) % 2]), ((n - 1) / 2) & 1, p.flags);
+        red[(3 * kShare + nth) * kRows + r] = l;
+        red[(4 * kShare + nth) * kRows + r] = pm;
+        ok = share_sync_and(warp, ok && w && !failed);
+        l = pm = 0.0f;
+#pragma unroll
+        for (uint32_t k = 0; k < kShare; k++) {
+            l += red[(3 * kShare + k) * kRows + r];
+            pm += red[(4 * kShare + k) * kRows + r];
+        }
         if (!ok) s_fail = 1;
         tc_fence_after();
         float* part = p.part + (((uint64_t)blockIdx.x * p.c.kv_heads + kvh) * p.splits +
                                 blockIdx.z) * ((HD + 2) * kRows);
         const float by = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll 1
-        for (uint32_t c = 0; c < HD / 32; c++) {
-            const uint32_t d = half * (HD / 2) + 16 * c;
+#pragma unroll
+        for (uint32_t c = 0; c < HD / (16 * kShare); c++) {
+            const uint32_t d = nth * (HD / kShare) + 16 * c;
             float o[16];
 #pragma unroll
             for (int k = 0; k < 16; k++) o[k] = 0.0f;
@@ -482,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     __stcg(part + (d + k) * kRows + r, o[k / 8 * 8 + 2 * (k % 4) + k % 8 / 4] + pm);
             }
         }
-        if (parts > 1 && half == 0) {
+        if (parts > 1 && nth == 0) {
             __stcg(part + HD * kRows + r, m_ref);
             __stcg(part + (HD + 1) * kRows + r, l);
         }
@@ -497,30 +553,29 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncthreads();
         if (s_last && tid < kSoftmax) {
-            const uint32_t r = tid % kRows, half = tid / kRows;
             const float* part = p.part + ((uint64_t)blockIdx.x * p.c.kv_heads + kvh) * p.splits *
                                              ((HD + 2) * kRows) + r;
-            float M = -INFINITY, L = 0.0f, y[HD / 2];
+            float M = -INFINITY, L = 0.0f, y[HD / kShare];
             for (uint32_t z = 0; z < parts; z++)
                 M = fmaxf(M, __ldcg(part + (z * (HD + 2) + HD) * kRows));
 #pragma unroll
-            for (uint32_t k = 0; k < HD / 2; k++) y[k] = 0.0f;
+            for (uint32_t k = 0; k < HD / kShare; k++) y[k] = 0.0f;
             for (uint32_t z = 0; z < parts; z++) {
                 const float* pz = part + z * ((HD + 2) * kRows);
                 const float mz = __ldcg(pz + HD * kRows), lz = __ldcg(pz + (HD + 1) * kRows);
                 const float f = mz == -INFINITY ? 0.0f : ex2(mz - M);
                 L = fmaf(lz, f, L);
 #pragma unroll
-                for (uint32_t k = 0; k < HD / 2; k++)
-                    y[k] = fmaf(__ldcg(pz + (half * (HD / 2) + k) * kRows), f, y[k]);
+                for (uint32_t k = 0; k < HD / kShare; k++)
+                    y[k] = fmaf(__ldcg(pz + (nth * (HD / kShare) + k) * kRows), f, y[k]);
             }
             const float by = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
-            for (uint32_t c = 0; c < HD / 32; c++) {
+            for (uint32_t c = 0; c < HD / (16 * kShare); c++) {
                 float v[16];
 #pragma unroll
                 for (int k = 0; k < 16; k++) v[k] = y[16 * c + k] * by;
-                if (live) put_out(p, orow, half * (HD / 2) + 16 * c, v);
+                if (live) put_out(p, orow, nth * (HD / kShare) + 16 * c, v);
             }
         }
     }

@@ -32,6 +32,16 @@ __device__ __forceinline__ void tc_mma_bf16(uint32_t d, uint64_t a, uint64_t b, 
         "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(m)
         : "memory");
 }
+// D[tmem] (+)= A[tmem] x B[smem desc]^T: row i of A is lane i, two K elements a 32-bit column.
+__device__ __forceinline__ void tc_mma_bf16_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                               uint32_t accumulate) {
+    const uint32_t m = 0;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(m)
+        : "memory");
+}
 // D[tmem] (+)= A x B^T on the tf32 pipe (fp32 operands in shared memory, read as tf32).
 __device__ __forceinline__ void tc_mma_tf32(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                             uint32_t accumulate) {
@@ -96,6 +106,13 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float* v) {
         "r"(__float_as_uint(v[9])), "r"(__float_as_uint(v[10])), "r"(__float_as_uint(v[11])),
         "r"(__float_as_uint(v[12])), "r"(__float_as_uint(v[13])), "r"(__float_as_uint(v[14])),
         "r"(__float_as_uint(v[15]))
+        : "memory");
+}
+// 8 consecutive 32-bit columns into this thread's TMEM lane.
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
         : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() {
