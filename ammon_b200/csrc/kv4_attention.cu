@@ -52,8 +52,10 @@ constexpr uint32_t kTile = kWarps * kTurn;  // positions of one block's turn
 // 57.7 and 62.5 us at 64 ragged rows of up to 8192 positions (32 heads of 8 kv heads, head 128,
 // bf16), 63.8, 54.7, 54.6, 54.1 and 57.1 at 256 of up to 1024 (12 heads, head 64, f32).
 constexpr uint32_t kLead = 2;
-// Query slots of one kv head over one cache from which on tcgen05 takes them (bf16 outputs).
-constexpr uint64_t kTensorSlots = 64;
+// More query slots than these of a kv head over one cache go to tcgen05 (bf16 outputs; here against
+// there, 8 kv heads, head 128): 64 slots of 2048 positions 15 us against 24, 256 of 64 positions 9
+// against 14 and of 2000 32 against 26, 512 of 128 15 against 14, 2048 of 1024 89 against 33.
+constexpr uint64_t kTensorSlots = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Kv4AttnParams {
@@ -948,7 +950,7 @@ void record_kv4_attention(ab_scheme* s, const char* label, const float* q, uint3
         fail(AB_ERR_ARGUMENT, "kv4_attention: the scheme needs a runtime (it allocates the split "
                               "scratch)");
     const uint64_t slots = (uint64_t)rows * (heads / cache.kv_heads);  // over one shared cache
-    if (cache.row_stride == 0 && out_dtype == AB_BF16 && slots >= kTensorSlots &&
+    if (cache.row_stride == 0 && out_dtype == AB_BF16 && slots > kTensorSlots &&
         record_kv4_prompt_tc(s, label, q, rows, heads, cache, out, step))
         return;
     Kv4AttnParams p = {};

@@ -6,11 +6,11 @@
 // c - 8 is a whole number, exact in bf16, so the operands made from the cache lose nothing, and s
 // and m' enter per position, outside the products.
 //
-// One block takes 128 slots of a kv head over a run of 64-position tiles, a slot a TMEM lane:
+// One block takes 128 slots of a kv head over a run of 128-position tiles, a slot a TMEM lane:
 //  - warps 16-19 read a tile's codes (the next tile's are on their way meanwhile), write them as
 //    bf16 operands of K and V in the 128-byte-swizzled layout, and the tile's steps and offsets;
-//  - warp 20 (one thread) issues tcgen05.mma: S = Q.(K codes)^T into one of two 64-column TMEM
-//    buffers, a tile ahead, and O += P.(V codes), V being an MN-major operand of the same layout.
+//  - warp 20 (one thread) issues tcgen05.mma: S = Q.(K codes)^T into one of two TMEM buffers, a
+//    tile ahead, and O += P.(V codes), V being an MN-major operand of the same layout.
 //    Q and P are operands in TMEM: from shared memory, each product read 4 KB of them beside the
 //    2 or 4 KB of codes, which made shared memory the bound;
 //  - warps 0-15, four threads a slot, make scores of S, keep the slot's maximum and sums, write
@@ -23,11 +23,19 @@
 //
 // Few blocks split their tiles over several (as many as the device holds at once); the last one
 // to finish a slot block joins the parts in order.
+// Measured, 8 kv heads of 4 query heads, head 128: 256 rows over 2048 positions 35.5 us (the
+// mma.sync kernel of kv4_attention.cu takes 80), 1024 over 8192 346 us (867), of which a tile is
+// some 2.5 us: the weights' arithmetic, 16384 exponentials and the scales' broadcast reads, in
+// phases that all warps pass together; the products are a third of it. With 64-position tiles, P
+// beside S instead of in its place, 39 and 422 us; with Q and P in shared memory 43 and 460.
+// Starting and joining is about 11 us.
+//
 // Every wait is bounded; one that runs out raises the device flag, and the block still lets its
 // products finish and frees its TMEM.
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "internal.h"
@@ -40,17 +48,17 @@ namespace ab {
 namespace {
 
 constexpr uint32_t kRows = 128;      // slots of a block (TMEM lanes)
-constexpr uint32_t kTile = 64;       // positions
-constexpr uint32_t kStages = 4;      // tiles unpacked at a time
+constexpr uint32_t kTile = 128;      // positions
+constexpr uint32_t kStages = 3;      // tiles unpacked at a time
 constexpr uint32_t kShare = 4;       // threads of a slot
 constexpr uint32_t kCols = kTile / kShare;
 constexpr uint32_t kSoftmax = kRows * kShare;  // threads of warps 0-15
 constexpr uint32_t kUnpack = 128;              // of warps 16-19
 constexpr uint32_t kUnpackWarp = kSoftmax / 32, kMmaWarp = kUnpackWarp + kUnpack / 32;
 constexpr uint32_t kThreads = kSoftmax + kUnpack + 32;
-// Columns of TMEM: S twice, O, Q (value, rest), P (value, rest) twice.
-constexpr uint32_t kTmemCols = 512, kTmemO = 128, kTmemQ = 256, kTmemP = 384;
-constexpr uint32_t kMinTiles = 4;    // a part has at least so many
+// Columns of TMEM: S twice, each replaced by its P (value, rest), O, Q (value, rest).
+constexpr uint32_t kTmemCols = 512, kTmemO = 256, kTmemQ = 384;
+constexpr uint32_t kMinTiles = 2;    // a part has at least so many
 constexpr float kRescale = 11.5f;    // base 2: P stays below 2^kRescale steps of V
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -119,7 +127,8 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 __device__ __forceinline__ void split(float a, float b, uint32_t* value, uint32_t* rest) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     *value = *reinterpret_cast<const uint32_t*>(&h);
-    const float2 left = add2(make_float2(a, b), make_float2(-bf16lo(*value), -bf16hi(*value)));
+    const float2 left = fma2(make_float2(bf16lo(*value), bf16hi(*value)), make_float2(-1.0f, -1.0f),
+                             make_float2(a, b));
     const __nv_bfloat162 l = __floats2bfloat162_rn(left.x, left.y);
     *rest = *reinterpret_cast<const uint32_t*>(&l);
 }
@@ -139,6 +148,14 @@ __device__ __forceinline__ uint4 ld16(const uint32_t* p) {
                  : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
                  : "l"(p));
     return r;
+}
+// Asynchronous copy of 16 bytes, or zeros (size 0, nothing is read).
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t size) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(size)
+                 : "memory");
+}
+__device__ __forceinline__ void copies_wait_all() {
+    asm volatile("cp.async.wait_all;" ::: "memory");
 }
 // Sixteen dims from d on of an output row.
 __device__ __forceinline__ void put_out(const PromptParams& p, uint64_t orow, uint32_t d,
@@ -180,8 +197,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     using LY = Layout<HD>;
     constexpr uint32_t BOX = HD / 64;  // 64-dim blocks of a row
     extern __shared__ __align__(16) unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t full[kStages], empty[kStages], s_full[2], s_free[2], p_full[2],
-        pv_done[2], done;
+    __shared__ __align__(8) uint64_t full[kStages], empty[kStages], s_full[2], p_full[2], pv_done[2],
+        done;
     __shared__ uint32_t s_tmem, s_most[4];
     __shared__ int s_fail, s_last;
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -191,6 +208,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t kvh = blockIdx.y, slot = blockIdx.x * kRows + tid % kRows;
 
     pdl_wait();
+    // The queries, for now in the room of the later stages: whole rows a few lanes each (a row a
+    // thread, read where it is used, took 3 us).
+    float* staged = reinterpret_cast<float*>(smem + 2 * LY::T);
+    constexpr uint32_t STRIDE = HD + 4;
+    static_assert(kRows * STRIDE * 4 <= (kStages - 1) * 2 * LY::T);
+    if (tid < kSoftmax) {
+#pragma unroll
+        for (uint32_t i = tid; i < kRows * HD / 4; i += kSoftmax) {
+            const uint32_t d = i % (HD / 4) * 4, sl = blockIdx.x * kRows + i / (HD / 4);
+            const uint32_t in = sl / p.group;
+            float* to = staged + i / (HD / 4) * STRIDE + d;
+            const bool some = in < p.rows && d < p.c.head;
+            const float* from = p.q;
+            if (some)
+                from += ((uint64_t)in * p.heads + kvh * p.group + sl % p.group) * p.c.head + d;
+            if (p.qvec) {
+                copy16(smem_u32(to), from, some ? 16 : 0);
+            } else {
+#pragma unroll
+                for (uint32_t k = 0; k < 4; k++) to[k] = some && d + k < p.c.head ? from[k] : 0.0f;
+            }
+        }
+        copies_wait_all();
+    }
     // the slot's row, head and last position; each of its threads needs them
     const uint32_t row = slot / p.group;
     const bool live = tid < kSoftmax && row < p.rows;
@@ -222,7 +263,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (uint32_t i = 0; i < 2; i++) {
             mbar_init(smem_u32(&s_full[i]), 1);
-            mbar_init(smem_u32(&s_free[i]), kSoftmax);
             mbar_init(smem_u32(&p_full[i]), kSoftmax);
             mbar_init(smem_u32(&pv_done[i]), 1);
         }
@@ -231,6 +271,32 @@ __global__ void __launch_bounds__(kThreads, 1)
         s_fail = 0;
     }
     if (warp == 0) tmem_alloc(smem_u32(&s_tmem), kTmemCols);
+    // a tile's codes, a position a thread of the warps that unpack; the first are on their way
+    // while the queries are staged
+    const uint32_t line = tid % kUnpack;
+    const uint64_t head0 = (uint64_t)kvh * p.c.seq;
+    const uint32_t chunks = p.c.words / 4;
+    struct Raw {
+        uint4 w[2][2 * BOX];  // of K and V, 32 dims each
+        uint32_t sc[2];
+    };
+    auto read = [&](uint32_t tile, Raw& raw) {
+        const uint32_t pos = (t_lo + tile) * kTile + line;
+        const bool in = tile < n && pos < until;
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+#pragma unroll
+            for (uint32_t c = 0; c < 2 * BOX; c++) {
+                raw.w[x][c] = make_uint4(0, 0, 0, 0);
+                if (in && c < chunks)
+                    raw.w[x][c] = ld16(p.c.codes[x] + (head0 + pos) * p.c.words + 4 * c);
+            }
+            raw.sc[x] = 0;
+            if (in) raw.sc[x] = __ldcg(p.c.scales[x] + head0 + pos);
+        }
+    };
+    Raw raw;
+    if (warp >= kUnpackWarp && warp < kMmaWarp) read(0, raw);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -240,29 +306,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid < kSoftmax) {
         // the slot's queries times log2(e) / sqrt(head): this thread's dims
         const float by = kLog2e / sqrtf((float)p.c.head);
-        const float* q = p.q + orow * p.c.head;
         float sum = 0.0f;
 #pragma unroll
         for (uint32_t j = 0; j < HD / (16 * kShare); j++) {
             uint32_t value[8], rest[8];
 #pragma unroll
             for (uint32_t e = 0; e < 2; e++) {
-                const uint32_t d = nth * (HD / kShare) + 16 * j + 8 * e;
+                const float* q = staged + r * STRIDE + nth * (HD / kShare) + 16 * j + 8 * e;
                 float v[8];
 #pragma unroll
                 for (uint32_t k = 0; k < 8; k += 4) {
-                    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (limit >= 0 && d + k < p.c.head) {
-                        if (p.qvec) {
-                            x = *reinterpret_cast<const float4*>(q + d + k);
-                        } else {
-                            const uint32_t left = p.c.head - d - k;
-                            x.x = q[d + k];
-                            if (left > 1) x.y = q[d + k + 1];
-                            if (left > 2) x.z = q[d + k + 2];
-                            if (left > 3) x.w = q[d + k + 3];
-                        }
-                    }
+                    const float4 x = *reinterpret_cast<const float4*>(q + k);
                     v[k] = x.x * by;
                     v[k + 1] = x.y * by;
                     v[k + 2] = x.z * by;
@@ -286,66 +340,40 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     float m_ref = -INFINITY, l = 0.0f, pm = 0.0f;
     if (warp >= kUnpackWarp && warp < kMmaWarp) {
-        // ---- codes to operands: a thread half of a position's chunks (32 dims each) ----
-        const uint32_t u = tid - kSoftmax, line = u / 2, odd = u % 2;
-        const uint64_t head0 = (uint64_t)kvh * p.c.seq;
-        const uint32_t chunks = p.c.words / 4;
-        struct Raw {
-            uint4 w[2][BOX];
-            uint32_t sc;  // of K (even threads) or V
-        };
-        auto read = [&](uint32_t tile, Raw& raw) {
-            const uint32_t pos = (t_lo + tile) * kTile + line;
-            const bool in = tile < n && pos < until;
-#pragma unroll
-            for (int x = 0; x < 2; x++)
-#pragma unroll
-                for (uint32_t b = 0; b < BOX; b++) {
-                    const uint32_t c = 2 * b + odd;
-                    raw.w[x][b] = make_uint4(0, 0, 0, 0);
-                    if (in && c < chunks)
-                        raw.w[x][b] = ld16(p.c.codes[x] + (head0 + pos) * p.c.words + 4 * c);
-                }
-            raw.sc = 0;
-            if (in) raw.sc = __ldcg(p.c.scales[odd] + head0 + pos);
-        };
+        // ---- codes to operands: a position a thread ----
         auto write = [&](uint32_t i, const Raw& raw) {
             const uint32_t s = i % kStages;
             if (i >= kStages && !mbar_wait_bounded(smem_u32(&empty[s]), (i / kStages - 1) & 1,
                                                    p.flags))
                 return false;
             const uint32_t to = base + s * 2 * LY::T;
+            float* scales = reinterpret_cast<float*>(smem + LY::SCALES_AT) + s * (4 * kTile) + line;
 #pragma unroll
-            for (int x = 0; x < 2; x++)
+            for (int x = 0; x < 2; x++) {
 #pragma unroll
-                for (uint32_t b = 0; b < BOX; b++) {
-                    const uint4& w = raw.w[x][b];
+                for (uint32_t c = 0; c < 2 * BOX; c++) {
+                    const uint4& w = raw.w[x][c];
                     const uint32_t word[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                     for (uint32_t k = 0; k < 4; k++) {
                         uint32_t v[4];
                         unpack(word[k], v);
-                        put(to + x * LY::T + b * (kTile * 128) + row_chunk(line, 4 * odd + k), v);
+                        put(to + x * LY::T + c / 2 * (kTile * 128) +
+                                row_chunk(line, c % 2 * 4 + k),
+                            v);
                     }
                 }
-            float* scales =
-                reinterpret_cast<float*>(smem + LY::SCALES_AT) + (s * 2 + odd) * (2 * kTile) + line;
-            scales[0] = bf16lo(raw.sc);
-            scales[kTile] = fmaf(8.0f, bf16lo(raw.sc), bf16hi(raw.sc));
+                scales[2 * x * kTile] = bf16lo(raw.sc[x]);
+                scales[(2 * x + 1) * kTile] = fmaf(8.0f, bf16lo(raw.sc[x]), bf16hi(raw.sc[x]));
+            }
             fence_proxy_async_smem();
             mbar_arrive(smem_u32(&full[s]));
             return true;
         };
-        // two tiles are on their way
-        Raw even, uneven;
-        read(0, even);
-        read(1, uneven);
         bool ok = true;
-        for (uint32_t i = 0; i < n && ok; i += 2) {
-            ok = write(i, even);
-            read(i + 2, even);
-            if (ok && i + 1 < n) ok = write(i + 1, uneven);
-            read(i + 3, uneven);
+        for (uint32_t i = 0; i < n && ok; i++) {
+            ok = write(i, raw);
+            read(i + 1, raw);
         }
         if (!ok) s_fail = 1;
     } else if (warp == kMmaWarp) {
@@ -356,8 +384,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t s = i % kStages;
                 if (!mbar_wait_bounded(smem_u32(&full[s]), (i / kStages) & 1, p.flags))
                     return false;
-                // the tile before the last has been read out of this buffer
-                if (i >= 2 && !mbar_wait_bounded(smem_u32(&s_free[i % 2]), (i / 2 - 1) & 1, p.flags))
+                // its buffer holds the P before the last until that has been multiplied
+                if (i >= 2 &&
+                    !mbar_wait_bounded(smem_u32(&pv_done[i % 2]), (i / 2 - 1) & 1, p.flags))
                     return false;
                 tc_fence_after();
                 const uint32_t k_at = base + s * 2 * LY::T;
@@ -387,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 tc_fence_after();
                 const uint32_t v_at = base + (i % kStages * 2 + 1) * LY::T;
-                const uint32_t w = tmem + kTmemP + i % 2 * kTile;
+                const uint32_t w = tmem + i % 2 * kTile;
 #pragma unroll
                 for (uint32_t k = 0; k < kTile / 16; k++) {
                     const uint64_t vd = sw128_desc_mn(v_at + k * 16 * 128, kTile * 128);
@@ -411,39 +440,34 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (uint32_t i = 0; i < n; i++) {
             bool w = mbar_wait_bounded(smem_u32(&s_full[i % 2]), (i / 2) & 1, p.flags);
             w = mbar_wait_bounded(smem_u32(&full[i % kStages]), (i / kStages) & 1, p.flags) && w;
-            // this P has been multiplied
-            if (i >= 2)
-                w = mbar_wait_bounded(smem_u32(&pv_done[i % 2]), (i / 2 - 1) & 1, p.flags) && w;
             __syncwarp();
             tc_fence_after();
-            float xs[kCols];
-            tmem_ld16(mine + (i % 2) * kTile + nth * kCols, xs);
-            tc_fence_before();
-            mbar_arrive(smem_u32(&s_free[i % 2]));
             const float4* scales = reinterpret_cast<const float4*>(smem + LY::SCALES_AT) +
                                    i % kStages * kTile + nth * (kCols / 4);
-            float2 x[kCols / 2], vs[kCols / 2], vm[kCols / 2];
+            float2 x[kCols / 2];
 #pragma unroll
-            for (uint32_t j = 0; j < kCols / 4; j++) {
-                const float4 ks = scales[j], km = scales[kTile / 4 + j];
-                const float4 s4 = scales[2 * (kTile / 4) + j], m4 = scales[3 * (kTile / 4) + j];
-                x[2 * j] = fma2(make_float2(xs[4 * j], xs[4 * j + 1]), make_float2(ks.x, ks.y),
-                                mul2(qsum, make_float2(km.x, km.y)));
-                x[2 * j + 1] = fma2(make_float2(xs[4 * j + 2], xs[4 * j + 3]),
-                                    make_float2(ks.z, ks.w),
-                                    mul2(qsum, make_float2(km.z, km.w)));
-                vs[2 * j] = make_float2(s4.x, s4.y);
-                vs[2 * j + 1] = make_float2(s4.z, s4.w);
-                vm[2 * j] = make_float2(m4.x, m4.y);
-                vm[2 * j + 1] = make_float2(m4.z, m4.w);
+            for (uint32_t c = 0; c < kCols / 16; c++) {
+                float xs[16];
+                tmem_ld16(mine + (i % 2) * kTile + nth * kCols + 16 * c, xs);
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++) {
+                    const float4 ks = scales[4 * c + j], km = scales[kTile / 4 + 4 * c + j];
+                    x[8 * c + 2 * j] =
+                        fma2(make_float2(xs[4 * j], xs[4 * j + 1]), make_float2(ks.x, ks.y),
+                             mul2(qsum, make_float2(km.x, km.y)));
+                    x[8 * c + 2 * j + 1] =
+                        fma2(make_float2(xs[4 * j + 2], xs[4 * j + 3]), make_float2(ks.z, ks.w),
+                             mul2(qsum, make_float2(km.z, km.w)));
+                }
             }
+            tc_fence_before();
             // columns 0 .. seen are attended over; what the others hold is not used, NaN or not
             const int32_t seen = limit - (int32_t)((t_lo + i) * kTile + nth * kCols);
             if (seen < (int32_t)kCols - 1) {
 #pragma unroll
                 for (int j = 0; j < (int)kCols / 2; j++) {
-                    if (2 * j > seen) x[j].x = -INFINITY, vs[j].x = vm[j].x = 0.0f;
-                    if (2 * j + 1 > seen) x[j].y = -INFINITY, vs[j].y = vm[j].y = 0.0f;
+                    if (2 * j > seen) x[j].x = -INFINITY;
+                    if (2 * j + 1 > seen) x[j].y = -INFINITY;
                 }
             }
             float most = fmaxf(x[0].x, x[0].y);
@@ -453,6 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             maxima[nth * kRows] = most;
             ok = share_sync_and(warp, w && !failed);
             if (!ok) break;
+            tc_fence_after();  // the slot's S has been read: P may take its place
 #pragma unroll
             for (uint32_t k = 0; k < kShare; k++) most = fmaxf(most, maxima[k * kRows]);
             float alpha = 1.0f;
@@ -467,14 +492,28 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float m0 = m_ref == -INFINITY ? 0.0f : -m_ref;  // nothing seen: weights of 0
             const float2 m2 = make_float2(m0, m0);
             float2 sum = make_float2(0.0f, 0.0f), off = sum;
+            auto weigh = [&](auto masked) {
 #pragma unroll
-            for (uint32_t j = 0; j < kCols / 2; j++) {
-                const float2 y = add2(x[j], m2);
-                const float2 a = make_float2(ex2(y.x), ex2(y.y));
-                sum = add2(sum, a);
-                off = fma2(a, vm[j], off);
-                x[j] = mul2(a, vs[j]);
-            }
+                for (int j = 0; j < (int)kCols / 4; j++) {
+                    const float4 vs = scales[2 * (kTile / 4) + j], vm = scales[3 * (kTile / 4) + j];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        float2 s2 = e ? make_float2(vs.z, vs.w) : make_float2(vs.x, vs.y);
+                        float2 o2 = e ? make_float2(vm.z, vm.w) : make_float2(vm.x, vm.y);
+                        if constexpr (decltype(masked)::value) {
+                            if (4 * j + 2 * e > seen) s2.x = o2.x = 0.0f;
+                            if (4 * j + 2 * e + 1 > seen) s2.y = o2.y = 0.0f;
+                        }
+                        const float2 y = add2(x[2 * j + e], m2);
+                        const float2 a = make_float2(ex2(y.x), ex2(y.y));
+                        sum = add2(sum, a);
+                        off = fma2(a, o2, off);
+                        x[2 * j + e] = mul2(a, s2);
+                    }
+                }
+            };
+            if (seen < (int32_t)kCols - 1) weigh(std::true_type());
+            else weigh(std::false_type());
             l = fmaf(l, alpha, sum.x + sum.y);
             pm = fmaf(pm, alpha, off.x + off.y);
             // O is at rest once the tile before is in it
@@ -493,12 +532,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_st16(at, o);
                 }
             }
-            uint32_t value[8], rest[8];
 #pragma unroll
-            for (int k = 0; k < 8; k++) split(x[k].x, x[k].y, &value[k], &rest[k]);
-            const uint32_t at = mine + kTmemP + i % 2 * kTile + nth * (kCols / 2);
-            tmem_st8(at, value);
-            tmem_st8(at + kTile / 2, rest);
+            for (uint32_t c = 0; c < kCols / 2; c += 8) {
+                uint32_t value[8], rest[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) split(x[c + k].x, x[c + k].y, &value[k], &rest[k]);
+                const uint32_t at = mine + i % 2 * kTile + nth * (kCols / 2) + c;
+                tmem_st8(at, value);
+                tmem_st8(at + kTile / 2, rest);
+            }
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(smem_u32(&p_full[i % 2]));
@@ -534,8 +576,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (live) put_out(p, orow, d, y);
             } else {
 #pragma unroll
-                for (int k = 0; k < 16; k++)
-                    __stcg(part + (d + k) * kRows + r, o[k / 8 * 8 + 2 * (k % 4) + k % 8 / 4] + pm);
+                for (int k = 0; k < 16; k += 4) {
+                    const float* at = o + k / 8 * 8 + k % 8 / 4;
+                    __stcg(reinterpret_cast<float4*>(part) + (d + k) / 4 * kRows + r,
+                           make_float4(at[0] + pm, at[2] + pm, at[4] + pm, at[6] + pm));
+                }
             }
         }
         if (parts > 1 && nth == 0) {
@@ -554,27 +599,43 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncthreads();
         if (s_last && tid < kSoftmax) {
             const float* part = p.part + ((uint64_t)blockIdx.x * p.c.kv_heads + kvh) * p.splits *
-                                             ((HD + 2) * kRows) + r;
-            float M = -INFINITY, L = 0.0f, y[HD / kShare];
+                                             ((HD + 2) * kRows);
+            float M = -INFINITY, L = 0.0f;
+            float4 y[HD / (4 * kShare)];
+#pragma unroll 4
             for (uint32_t z = 0; z < parts; z++)
-                M = fmaxf(M, __ldcg(part + (z * (HD + 2) + HD) * kRows));
+                M = fmaxf(M, __ldcg(part + (z * (HD + 2) + HD) * kRows + r));
 #pragma unroll
-            for (uint32_t k = 0; k < HD / kShare; k++) y[k] = 0.0f;
+            for (uint32_t k = 0; k < HD / (4 * kShare); k++) y[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             for (uint32_t z = 0; z < parts; z++) {
                 const float* pz = part + z * ((HD + 2) * kRows);
-                const float mz = __ldcg(pz + HD * kRows), lz = __ldcg(pz + (HD + 1) * kRows);
+                float4 v[HD / (4 * kShare)];
+#pragma unroll
+                for (uint32_t k = 0; k < HD / (4 * kShare); k++)
+                    v[k] = __ldcg(reinterpret_cast<const float4*>(pz) +
+                                  (nth * (HD / (4 * kShare)) + k) * kRows + r);
+                const float mz = __ldcg(pz + HD * kRows + r), lz = __ldcg(pz + (HD + 1) * kRows + r);
                 const float f = mz == -INFINITY ? 0.0f : ex2(mz - M);
                 L = fmaf(lz, f, L);
 #pragma unroll
-                for (uint32_t k = 0; k < HD / kShare; k++)
-                    y[k] = fmaf(__ldcg(pz + (nth * (HD / kShare) + k) * kRows), f, y[k]);
+                for (uint32_t k = 0; k < HD / (4 * kShare); k++) {
+                    y[k].x = fmaf(v[k].x, f, y[k].x);
+                    y[k].y = fmaf(v[k].y, f, y[k].y);
+                    y[k].z = fmaf(v[k].z, f, y[k].z);
+                    y[k].w = fmaf(v[k].w, f, y[k].w);
+                }
             }
             const float by = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
             for (uint32_t c = 0; c < HD / (16 * kShare); c++) {
                 float v[16];
 #pragma unroll
-                for (int k = 0; k < 16; k++) v[k] = y[16 * c + k] * by;
+                for (int k = 0; k < 4; k++) {
+                    v[4 * k] = y[4 * c + k].x * by;
+                    v[4 * k + 1] = y[4 * c + k].y * by;
+                    v[4 * k + 2] = y[4 * c + k].z * by;
+                    v[4 * k + 3] = y[4 * c + k].w * by;
+                }
                 if (live) put_out(p, orow, nth * (HD / kShare) + 16 * c, v);
             }
         }

@@ -23,7 +23,7 @@ def query(rng, *shape):
 @pytest.mark.parametrize("last", [63, 64, 700])
 def test_prompt_rows(rt, heads, kv, head, last):
     rng = np.random.default_rng(heads * 100 + head + last)
-    rows = max(64 // (heads // kv), 40) + 3
+    rows = 260 // (heads // kv) + 3
     first = max(0, last + 1 - rows)
     positions = [min(last, first + i) for i in range(rows)]
     layer = packed(rng, (), kv, last + 2, head)
@@ -58,7 +58,7 @@ def test_prompt_positions_in_any_order_and_past_the_end(rt):
 def test_prompt_over_rows_that_are_not_finite(rt):
     """A key or value vector that is NaN reaches exactly the rows at or past its position."""
     rng = np.random.default_rng(32)
-    heads, kv, head, rows, seq = 8, 4, 64, 80, 200
+    heads, kv, head, rows, seq = 16, 4, 64, 80, 200
     for which in (1, 3):
         layer = packed(rng, (), kv, seq, head)
         positions = list(range(100, 180))
@@ -67,7 +67,8 @@ def test_prompt_over_rows_that_are_not_finite(rt):
         q = query(rng, rows, heads, head)
         got = attend(rt, q, layer, positions, ab.BF16)
         nan = np.isnan(got)
-        assert nan[50:, 2:4].all() and not nan[:50].any() and not nan[:, [0, 1, 4, 5, 6, 7]].any()
+        assert nan[50:, 4:8].all() and not nan[:50].any()
+        assert not nan[:, :4].any() and not nan[:, 8:].any()
     layer = packed(rng, (), kv, seq, head)
     q[7, 3, 5], q[9, 6, 0] = np.nan, np.inf
     nan = np.isnan(attend(rt, q, layer, positions, ab.BF16))
@@ -81,7 +82,7 @@ def test_prompt_where_maxima_grow_along_the_cache(rt):
     """Scores that rise by thousands over the positions move every running maximum; the weights'
     own order of size changes with the steps of V."""
     rng = np.random.default_rng(33)
-    heads, kv, head, rows, seq = 4, 1, 64, 64, 640
+    heads, kv, head, rows, seq = 4, 1, 64, 90, 640
     k = rng.standard_normal((kv, seq, head)).astype(np.float32)
     k *= np.linspace(0.01, 40, seq, dtype=np.float32)[None, :, None]
     v = rng.standard_normal((kv, seq, head)).astype(np.float32)
@@ -95,7 +96,7 @@ def test_prompt_where_maxima_grow_along_the_cache(rt):
     rt.synchronize()
 
 
-@pytest.mark.parametrize("heads,kv,rows,last", [(2, 1, 64, 40000), (8, 8, 64, 9000),
+@pytest.mark.parametrize("heads,kv,rows,last", [(8, 1, 64, 40000), (4, 4, 300, 9000),
                                                 (4, 4, 1500, 1600)])
 def test_prompt_split_and_not(rt, heads, kv, rows, last):
     """One slot block over a long cache (a hundred parts), a few, and more blocks than the device
@@ -115,7 +116,7 @@ def test_prompt_replays_at_changing_positions(rt):
     """One recorded call whose rows move, so that its parts are one, some and none of theirs; beside
     it a call of another kind that uses the same scratch."""
     rng = np.random.default_rng(34)
-    heads, kv, head, rows, seq = 8, 2, 128, 40, 3000
+    heads, kv, head, rows, seq = 8, 2, 128, 70, 3000
     layer = packed(rng, (), kv, seq, head)
     q, q1 = query(rng, rows, heads, head), query(rng, 1, heads, head)
     up = upload(rt, layer)
@@ -127,7 +128,7 @@ def test_prompt_replays_at_changing_positions(rt):
     kernel.record(s, "one", ab.Tensor.from_array(rt, q1), up, out1, parcel1)
     kernel.record(s, "prompt", ab.Tensor.from_array(rt, q), up, out, parcel)
     kernel.record(s, "one", ab.Tensor.from_array(rt, q1), up, out1, parcel1)
-    for first in (0, 2960, 500, 25, 1900):
+    for first in (0, 2930, 500, 25, 1900):
         positions = [first + i for i in range(rows)]
         rt.deposit(parcel, [ab.DecodeStep(0, p) for p in positions])
         rt.deposit(parcel1, [ab.DecodeStep(0, first)])
@@ -142,7 +143,7 @@ def test_prompt_replays_at_changing_positions(rt):
 @pytest.mark.parametrize("head", [128, 72, 50])
 def test_prompt_at_odd_addresses(rt, head):
     rng = np.random.default_rng(35)
-    rows, heads, kv, seq = 33, 4, 2, 333
+    rows, heads, kv, seq = 33, 32, 2, 333
     positions = list(range(300, 333))
     layer = packed(rng, (), kv, seq, head)
     q = query(rng, rows, heads, head)
