@@ -16,9 +16,13 @@
 // fp16, the whole number and the rest, together 22 bits. So f32 results keep their digits, and one
 // lane's accumulators all belong to one head: its maximum, sum and rescaling need no exchange.
 //
-// Bound: the packed bytes. A warp's 32 positions (head 128) are 4352 bytes and about 400
-// instructions; a twelfth of them is mma. Each warp keeps the next 32 positions on their way into
-// shared memory while it computes on the present ones.
+// Bound: the packed bytes, and before them the instructions: a warp's 32 positions (head 128) are
+// 4352 bytes and about 470 instructions, 32 of them mma. Each warp keeps the next 32 positions on
+// their way into shared memory while it computes on the present ones. Measured (8 kv heads of 4
+// query heads, head 128): one row of 131072 positions 36.3 us (143 MB, 3.9 TB/s, half the issue
+// slots used); 64 rows of 1 to 8192, 56 us (265 MB, 4.7 TB/s); one of 8001, 10.3 us. 256 rows of 1 to
+// 1024 positions of 12 heads of 64 take 55 us (113 MB, 2.1 TB/s): 10 units a block, whose starts
+// and joins are what its barriers wait for.
 //
 // Split: the tiles (a turn of all warps of a block) of all units (a row's or a slot block's
 // positions of one kv head) form one line that the blocks of one wave share equally, so rows of
@@ -43,8 +47,8 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
-// Blocks of an SM. A third one (80 registers) measured 43 us instead of 37 at one row of 128k
-// positions, 70 instead of 73 at 256 rows of 512; one of 16 warps 37 and 101.
+// Blocks of an SM. A third one (80 registers) measured 43 us where two took 37 at one row of 128k
+// positions, 70 where two took 73 at 256 rows of 1 to 1024 (before kLead); one of 16 warps 37 and 101.
 constexpr int kResident = 2;
 constexpr uint32_t kTurn = 32;              // positions of one warp's turn
 constexpr uint32_t kTile = kWarps * kTurn;  // positions of one block's turn
