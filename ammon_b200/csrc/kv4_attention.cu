@@ -1003,6 +1003,9 @@ extern "C" int ab_kernel_kv4_attention(ab_scheme* s, ab_tensor q, const ab_kv4_l
                     std::to_string((uint64_t)rows * heads * head) +
                     " elements ([batch, heads * head]), got " + shape_str(out));
         expect_step(step, rows);
+        const uintptr_t q0 = (uintptr_t)q.data, o0 = (uintptr_t)out.data;
+        if (q0 < o0 + numel(out) * dtype_size(out.dtype) && o0 < q0 + numel(q) * 4)
+            invalid("parameter `out`: overlaps q");
         record_kv4_attention(s, "kv4_attention", (const float*)q.data, rows, heads, c, out.data,
                              out.dtype, (const Step*)step.data);
     });

@@ -241,8 +241,8 @@ int ab_kernel_kv4_load(ab_scheme* s, const ab_kv4_layer* cache, ab_tensor step, 
  * any whole number of query heads per kv head. With a batch dim each row has a cache of its
  * own; without one all rows attend over the same cache, each up to its own position (the rows
  * of a prompt). A row at a position >= seq gives zeros and raises AB_ERR_DEVICE. Positions
- * past a row's own are never used, whatever they hold. Scratch is allocated here and owned by
- * the scheme, which therefore needs a runtime. */
+ * past a row's own are never used, whatever they hold. out must not overlap q. Scratch is
+ * allocated here and owned by the scheme, which therefore needs a runtime. */
 int ab_kernel_kv4_attention(ab_scheme* s, ab_tensor q, const ab_kv4_layer* cache, ab_tensor out,
                             ab_tensor step);
 

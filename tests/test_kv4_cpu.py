@@ -143,3 +143,15 @@ def test_more_vectors_than_a_call_takes_are_refused(scheme):
         scheme, "s", many, many, layer(kv=8, words=4), step(1 << 28)), "too many vectors")
     refused(scheme, lambda: K.Kv4LoadKernel.prepare(None).record(
         scheme, "l", layer(kv=8, seq=1 << 28, words=4), step(), many, many), "too many vectors")
+
+
+def test_attention_onto_its_own_queries_is_refused(scheme):
+    k = K.Kv4AttentionKernel.prepare(None)
+    q = fake((3, 8, 64))
+    for out in (fake((3, 512)), fake((3, 512), ab.BF16, FAKE + 3 * 512 * 4 - 2),
+                fake((3, 512), ab.F32, FAKE - 4)):
+        refused(scheme, lambda: k.record(scheme, "a", q, layer(), out, step(3)), "overlaps q")
+    # beside them: refused for the runtime that a scheme of no device lacks, not for this
+    for ptr in (FAKE - 3 * 512 * 4, FAKE + 3 * 512 * 4):
+        refused(scheme, lambda: k.record(scheme, "a", q, layer(), fake((3, 512), ab.F32, ptr),
+                                         step(3)), "runtime", cls=ab.AmmonError)
