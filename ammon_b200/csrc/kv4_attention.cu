@@ -21,7 +21,7 @@
 // their way into shared memory while it computes on the present ones. Measured (8 kv heads of 4
 // query heads, head 128): one row of 131072 positions 36.3 us (143 MB, 3.9 TB/s, half the issue
 // slots used); 64 rows of 1 to 8192, 56 us (265 MB, 4.7 TB/s); one of 8001, 10.3 us. 256 rows of 1 to
-// 1024 positions of 12 heads of 64 take 55 us (113 MB, 2.1 TB/s): 10 units a block, whose starts
+// 1024 positions of 12 heads of 64 take 43 us (113 MB, 2.6 TB/s): five units a block, whose starts
 // and joins are what its barriers wait for.
 //
 // Split: the tiles (a turn of all warps of a block) of all units (a row's or a slot block's
@@ -45,17 +45,21 @@ namespace ab {
 
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
-// Blocks of an SM. A third one (80 registers) measured 43 us where two took 37 at one row of 128k
-// positions, 70 where two took 73 at 256 rows of 1 to 1024 (before kLead); one of 16 warps 37 and 101.
-constexpr int kResident = 2;
-constexpr uint32_t kTurn = 32;              // positions of one warp's turn
-constexpr uint32_t kTile = kWarps * kTurn;  // positions of one block's turn
-// Tiles that a unit is taken to cost beyond its own: 0, 1, 2, 3 and 8 measured 69.5, 59.1, 56.4,
-// 57.7 and 62.5 us at 64 ragged rows of up to 8192 positions (32 heads of 8 kv heads, head 128,
-// bf16), 63.8, 54.7, 54.6, 54.1 and 57.1 at 256 of up to 1024 (12 heads, head 64, f32).
-constexpr uint32_t kLead = 2;
+// Warps of an SM, in two blocks of eight (NW below) or, for units of four slots that outnumber
+// the small blocks, four of four: units start and end without the other blocks' waiting. Eight
+// warps against four, own caches of rows of 1 to so many positions, 32 heads of 8 kv heads, head
+// 128, bf16: 512 rows of 200 54 us against 40, 256 of 1000 53 against 45, 128 of 4000 64 against 58,
+// but 64 of 8192 (512 units) 56 against 60, one of 131072 36 against 41 (f32): with long stretches
+// there are twice the parts to join. A third block of eight (80 registers) measured 43 us where
+// two took 37 at one row of 128k positions; one of 16 warps 37, and 101 where two took 73 at 256
+// rows of 12 heads.
+constexpr int kSmWarps = 16;
+constexpr uint32_t kTurn = 32;  // positions of one warp's turn; a tile is one of a block's warps
+// Tiles that a unit is taken to cost beyond its own. Eight warps: 0, 1, 2, 3 and 8 measured 69.5,
+// 59.1, 56.4, 57.7 and 62.5 us at 64 ragged rows of up to 8192 positions (as above). Four: 2, 3
+// and 4 measured 43.7, 42.9 and 43.3 at 256 of up to 1024 (12 heads, head 64, f32).
+template <int NW>
+constexpr uint32_t kLead = NW == 8 ? 2 : 3;
 // More query slots than these of a kv head over one cache go to tcgen05 (bf16 outputs; here against
 // there, 8 kv heads, head 128): 64 slots of 2048 positions 15 us against 24, 256 of 64 positions 9
 // against 14 and of 2000 32 against 26, 512 of 128 15 against 14, 2048 of 1024 89 against 33.
@@ -205,8 +209,9 @@ __device__ __forceinline__ uint32_t item_length(const Kv4AttnParams& p, uint32_t
     return n;
 }
 // Tiles of the line; at least one, so that a row without positions is written too.
+template <int NW>
 __device__ __forceinline__ uint32_t tiles_of(uint32_t length) {
-    return max(1u, (length + kTile - 1) / kTile);
+    return max(1u, (length + NW * kTurn - 1) / (NW * kTurn));
 }
 
 // The line of `total` tiles over `blocks` blocks: the first `more` of them take one tile more.
@@ -292,13 +297,13 @@ struct Unit {
 // (what is left of the threads rests). A thread joins its parts as an online softmax does, so
 // that weights and values are read in one round, AHEAD parts at a time. so, sm, sl: the block's
 // shared arrays, free by now.
-template <int W, uint32_t S, typename OT>
+template <int W, int NW, uint32_t S, typename OT>
 __device__ __forceinline__ void join_parts(const Unit<W, S, OT>& unit, uint32_t first, uint32_t n,
                                         uint32_t tid, float* so, float (*sm)[S],
                                            float (*sl)[S]) {
     constexpr uint32_t PART = S * (32 * W + 2), COLS = S * 8 * W;
-    constexpr uint32_t JG = kThreads / COLS;
-    static_assert(JG >= 1 && JG <= kWarps, "exchanged values fit where the warps' parts were");
+    constexpr uint32_t JG = NW * 32 / COLS;
+    static_assert(JG >= 1 && JG <= NW, "exchanged values fit where the warps' parts were");
     constexpr uint32_t AHEAD = 8;
     const uint32_t col = tid % COLS, jg = tid / COLS;
     const uint32_t s = col / (8 * W);
@@ -348,10 +353,12 @@ __device__ __forceinline__ void join_parts(const Unit<W, S, OT>& unit, uint32_t 
     if (jg == 0) unit.write(col, x, L);
 }
 
-// W: words of codes in a quarter row (head up to 32 W). NT: four query slots each.
-template <int W, int NT, typename OT>
-__global__ void __launch_bounds__(kThreads, kResident)
+// W: words of codes in a quarter row (head up to 32 W). NT: four query slots each. NW: warps.
+template <int W, int NT, int NW, typename OT>
+__global__ void __launch_bounds__(NW * 32, kSmWarps / NW)
     kv4_attention_kernel(const __grid_constant__ Kv4AttnParams p) {
+    constexpr int kWarps = NW, kThreads = NW * 32;
+    constexpr uint32_t kTile = NW * kTurn;  // positions of one block's turn
     constexpr uint32_t S = 4 * NT;
     constexpr uint32_t HP = 32 * W;
     constexpr uint32_t ROW = 16 * W;  // bytes of a row of codes
@@ -394,11 +401,11 @@ __global__ void __launch_bounds__(kThreads, kResident)
     }
     uint32_t total = 0;  // tiles in all
     if (p.items == 1) {
-        if (warp == 0) total = (tiles_of(item_length<S>(p, 0)) + p.lead) * p.per_item;
+        if (warp == 0) total = (tiles_of<NW>(item_length<S>(p, 0)) + p.lead) * p.per_item;
     } else {
         uint32_t sum = 0;
         for (uint32_t i = tid; i < p.items; i += kThreads)
-            sum += tiles_of(item_length<S>(p, i)) + p.lead;
+            sum += tiles_of<NW>(item_length<S>(p, i)) + p.lead;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) s_scan[warp] = sum;
@@ -426,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, kResident)
         for (uint32_t i0 = 0; i0 < p.items; i0 += kThreads) {
             const uint32_t i = i0 + tid;
             const uint32_t n =
-                i < p.items ? (tiles_of(item_length<S>(p, i)) + p.lead) * p.per_item : 0;
+                i < p.items ? (tiles_of<NW>(item_length<S>(p, i)) + p.lead) * p.per_item : 0;
             uint32_t upto = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -460,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, kResident)
     if (warp == 0) {
         len = item_length<S>(p, item);
         len1 = item + 1 < p.items ? item_length<S>(p, item + 1) : 0;
-        n_tiles = tiles_of(len);
+        n_tiles = tiles_of<NW>(len);
     }
     auto plan = [&](uint32_t at, Span& span) {  // the unit at `at`: the first warp's work
         while (at - item_at >= (n_tiles + p.lead) * p.per_item) {
@@ -468,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, kResident)
             item++;
             len = len1;
             len1 = item + 1 < p.items ? item_length<S>(p, item + 1) : 0;
-            n_tiles = tiles_of(len);
+            n_tiles = tiles_of<NW>(len);
         }
         const uint32_t nth = (at - item_at) / (n_tiles + p.lead);
         if (lane == 0) {
@@ -874,31 +881,31 @@ __global__ void __launch_bounds__(kThreads, kResident)
     __syncthreads();
     for (uint32_t k = 0; k < s_jobs; k++) {
         const Job& job = s_job[k];
-        join_parts<W, S>(Unit<W, S, OT>{p, job.item, job.kvh, job.sub}, job.first, job.parts,
+        join_parts<W, NW>(Unit<W, S, OT>{p, job.item, job.kvh, job.sub}, job.first, job.parts,
                          tid, so, s_m, s_l);
         __syncthreads();
     }
 }
 
-template <int W, int NT, typename OT>
+template <int W, int NT, int NW, typename OT>
 void record_one(ab_scheme* s, const char* label, Kv4AttnParams p) {
-    constexpr uint32_t S = 4 * NT, PART = S * (32 * W + 2);
-    constexpr size_t smem = kWarps * (kStages * Stage<W>::BYTES + S * 32 * W * 4) +
+    constexpr uint32_t S = 4 * NT, PART = S * (32 * W + 2), TILE = NW * kTurn;
+    constexpr size_t smem = NW * (kStages * Stage<W>::BYTES + S * 32 * W * 4) +
                             2 * NT * W * 2 * 32 * sizeof(uint2);
-    auto* kernel = kv4_attention_kernel<W, NT, OT>;
+    auto* kernel = kv4_attention_kernel<W, NT, NW, OT>;
     const uint64_t units = (uint64_t)p.items * p.per_item;
-    const uint64_t tiles = units * ((p.c.seq + kTile - 1) / kTile);
-    if ((tiles + kLead * units) >> 31) invalid("kv4_attention: too much work for one call");
+    const uint64_t tiles = units * ((p.c.seq + TILE - 1) / TILE);
+    if ((tiles + kLead<NW> * units) >> 31) invalid("kv4_attention: too much work for one call");
     s->rt->activate();
     cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
                "kv4_attention shared memory");
     const uint32_t grid =
-        (uint32_t)std::min<uint64_t>((uint64_t)s->rt->sm_count * kResident, tiles);
+        (uint32_t)std::min<uint64_t>((uint64_t)s->rt->sm_count * (kSmWarps / NW), tiles);
     // with fewer units than blocks a stretch holds one or two: no difference, or 1 us lost
-    p.lead = units > grid ? kLead : 0;
+    p.lead = units > grid ? kLead<NW> : 0;
     kv4_take_scratch(s, (uint64_t)grid * 2 * PART * 4, units, &p.part, &p.tickets);
     s->add(label, [=](cudaStream_t stream) {
-        return launch(stream, dim3(grid), dim3(kThreads), smem, true, kernel, p);
+        return launch(stream, dim3(grid), dim3(NW * 32), smem, true, kernel, p);
     });
 }
 
@@ -912,10 +919,12 @@ void record_width(ab_scheme* s, const char* label, Kv4AttnParams p, int32_t out_
     p.items = p.shared ? blocks : p.rows;
     p.per_item = p.c.kv_heads * (p.shared ? 1 : blocks);
     const bool f32 = out_dtype == AB_F32;
-    if (S == 4)
-        f32 ? record_one<W, 1, float>(s, label, p) : record_one<W, 1, bf16>(s, label, p);
+    if (S == 8)
+        f32 ? record_one<W, 2, 8, float>(s, label, p) : record_one<W, 2, 8, bf16>(s, label, p);
+    else if ((uint64_t)p.items * p.per_item > (uint64_t)s->rt->sm_count * (kSmWarps / 4))
+        f32 ? record_one<W, 1, 4, float>(s, label, p) : record_one<W, 1, 4, bf16>(s, label, p);
     else
-        f32 ? record_one<W, 2, float>(s, label, p) : record_one<W, 2, bf16>(s, label, p);
+        f32 ? record_one<W, 1, 8, float>(s, label, p) : record_one<W, 1, 8, bf16>(s, label, p);
 }
 
 }  // namespace

@@ -227,3 +227,29 @@ def test_offsets_past_32_bits(rt):
         assert np.array_equal(back[i].read(), want.astype(np.float32))
     rt.synchronize()
     cache.close()
+
+
+@pytest.mark.parametrize("heads,kv,head,out_dtype", [(4, 1, 128, ab.BF16), (4, 2, 33, ab.F32),
+                                                     (3, 1, 96, ab.F32), (2, 2, 20, ab.BF16)])
+def test_attention_of_many_short_rows(rt, heads, kv, head, out_dtype):
+    """More units of up to four query heads than the device holds small blocks; lengths about the
+    tiles' and turns' ends, rows that fill several tiles among them, one past the end."""
+    rng = np.random.default_rng(heads * 1000 + head)
+    rows, seq = 650, 400
+    positions = rng.integers(0, 40, rows)
+    positions[::50] = [0, 31, 32, 127, 128, 129, 255, 256, 383, 384, 399, 63, 1]
+    positions[1::50] = 399
+    layer = packed(rng, (rows,), kv, seq, head)
+    q = rng.standard_normal((rows, heads, head)).astype(np.float32)
+    got = attend(rt, q, layer, positions, out_dtype)
+    check_attention(got, q, layer, positions, out_dtype, False)
+    assert np.array_equal(got, attend(rt, q, layer, positions, out_dtype))
+    bad = positions.copy()
+    bad[333] = seq
+    other = attend(rt, q, layer, bad, out_dtype, past_the_end=True)
+    assert (other[333] == 0).all()
+    # where the line's stretches end moves with the lengths, and with them the order of sums
+    keep = np.arange(rows) != 333
+    check_attention(other[keep], q[keep], [a[keep] for a in layer], positions[keep], out_dtype,
+                    False)
+    rt.synchronize()
