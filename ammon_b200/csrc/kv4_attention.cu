@@ -45,14 +45,15 @@ namespace ab {
 
 namespace {
 
-// Warps of an SM, in two blocks of eight (NW below) or, for units of four slots that outnumber
-// the small blocks, four of four: units start and end without the other blocks' waiting. Eight
-// warps against four, own caches of rows of 1 to so many positions, 32 heads of 8 kv heads, head
-// 128, bf16: 512 rows of 200 54 us against 40, 256 of 1000 53 against 45, 128 of 4000 64 against 58,
-// but 64 of 8192 (512 units) 56 against 60, one of 131072 36 against 41 (f32): with long stretches
-// there are twice the parts to join. A third block of eight (80 registers) measured 43 us where
-// two took 37 at one row of 128k positions; one of 16 warps 37, and 101 where two took 73 at 256
-// rows of 12 heads.
+// Warps of an SM, in two blocks of eight (NW below) or, for units that outnumber the small blocks,
+// four of four: units start and end without the other blocks' waiting. Eight warps against four,
+// own caches of rows of 1 to so many positions, 32 heads of 8 kv heads, head 128, bf16: 512 rows of
+// 200 54 us against 40, 256 of 1000 53 against 45, 128 of 4000 64 against 58, but 64 of 8192 (512
+// units) 56 against 60, one of 131072 36 against 41 (f32): with long stretches there are twice the
+// parts to join. Of eight slots a unit at head 97 to 128 only three small blocks fit an SM's shared
+// memory: 256 rows of 2000, 64 heads of 8, 107 us against 131, so it is eight warps there. A third
+// block of eight (80 registers) measured 43 us where two took 37 at one row of 128k positions; one
+// of 16 warps 37, and 101 where two took 73 at 256 rows of 12 heads.
 constexpr int kSmWarps = 16;
 constexpr uint32_t kTurn = 32;  // positions of one warp's turn; a tile is one of a block's warps
 // Tiles that a unit is taken to cost beyond its own. Eight warps: 0, 1, 2, 3 and 8 measured 69.5,
@@ -302,55 +303,59 @@ __device__ __forceinline__ void join_parts(const Unit<W, S, OT>& unit, uint32_t 
                                         uint32_t tid, float* so, float (*sm)[S],
                                            float (*sl)[S]) {
     constexpr uint32_t PART = S * (32 * W + 2), COLS = S * 8 * W;
-    constexpr uint32_t JG = NW * 32 / COLS;
-    static_assert(JG >= 1 && JG <= NW, "exchanged values fit where the warps' parts were");
+    constexpr uint32_t THREADS = NW * 32, JG = COLS < THREADS ? THREADS / COLS : 1;
+    static_assert(JG <= NW, "exchanged values fit where the warps' parts were");
     constexpr uint32_t AHEAD = 8;
-    const uint32_t col = tid % COLS, jg = tid / COLS;
-    const uint32_t s = col / (8 * W);
-    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float J = -INFINITY, L = 0.0f;
-    auto join = [&](const float4& v, float mj, float lj) {
-        if (mj == -INFINITY) return;
-        const float to = fmaxf(J, mj), a = ex2(J - to), b = ex2(mj - to);
-        x.x = fmaf(v.x, b, x.x * a);
-        x.y = fmaf(v.y, b, x.y * a);
-        x.z = fmaf(v.z, b, x.z * a);
-        x.w = fmaf(v.w, b, x.w * a);
-        L = fmaf(lj, b, L * a);
-        J = to;
-    };
-    for (uint32_t j0 = jg < JG ? jg : n; j0 < n; j0 += AHEAD * JG) {
-        float4 v[AHEAD];
-        float mj[AHEAD], lj[AHEAD];
+#pragma unroll 1
+    for (uint32_t c0 = 0; c0 < COLS; c0 += THREADS) {  // once, but with few threads
+        const uint32_t col = COLS < THREADS ? tid % COLS : c0 + tid;
+        const uint32_t jg = COLS < THREADS ? tid / COLS : (col < COLS ? 0 : 1);
+        const uint32_t s = col / (8 * W);
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float J = -INFINITY, L = 0.0f;
+        auto join = [&](const float4& v, float mj, float lj) {
+            if (mj == -INFINITY) return;
+            const float to = fmaxf(J, mj), a = ex2(J - to), b = ex2(mj - to);
+            x.x = fmaf(v.x, b, x.x * a);
+            x.y = fmaf(v.y, b, x.y * a);
+            x.z = fmaf(v.z, b, x.z * a);
+            x.w = fmaf(v.w, b, x.w * a);
+            L = fmaf(lj, b, L * a);
+            J = to;
+        };
+        for (uint32_t j0 = jg < JG ? jg : n; j0 < n; j0 += AHEAD * JG) {
+            float4 v[AHEAD];
+            float mj[AHEAD], lj[AHEAD];
 #pragma unroll
-        for (uint32_t u = 0; u < AHEAD; u++) {
-            const uint32_t j = j0 + u * JG;
-            // the unit begins inside the first block's stretch and before the others'
-            const float* pj = unit.p.part + ((uint64_t)2 * (first + j) + (j == 0)) * PART;
-            mj[u] = -INFINITY;
-            if (j < n) {
-                mj[u] = __ldcg(pj + COLS * 4 + s);
-                lj[u] = __ldcg(pj + COLS * 4 + S + s);
-                v[u] = __ldcg(reinterpret_cast<const float4*>(pj) + col);
+            for (uint32_t u = 0; u < AHEAD; u++) {
+                const uint32_t j = j0 + u * JG;
+                // the unit begins inside the first block's stretch and before the others'
+                const float* pj = unit.p.part + ((uint64_t)2 * (first + j) + (j == 0)) * PART;
+                mj[u] = -INFINITY;
+                if (j < n) {
+                    mj[u] = __ldcg(pj + COLS * 4 + s);
+                    lj[u] = __ldcg(pj + COLS * 4 + S + s);
+                    v[u] = __ldcg(reinterpret_cast<const float4*>(pj) + col);
+                }
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < AHEAD; u++) join(v[u], mj[u], lj[u]);
+        }
+        if constexpr (JG > 1) {
+            if (jg < JG) {
+                reinterpret_cast<float4*>(so)[jg * COLS + col] = x;
+                sm[jg][s] = J;  // the same from every thread of a slot
+                sl[jg][s] = L;
+            }
+            __syncthreads();
+            if (jg == 0) {
+#pragma unroll
+                for (uint32_t g = 1; g < JG; g++)
+                    join(reinterpret_cast<const float4*>(so)[g * COLS + col], sm[g][s], sl[g][s]);
             }
         }
-#pragma unroll
-        for (uint32_t u = 0; u < AHEAD; u++) join(v[u], mj[u], lj[u]);
+        if (jg == 0) unit.write(col, x, L);
     }
-    if constexpr (JG > 1) {
-        if (jg < JG) {
-            reinterpret_cast<float4*>(so)[jg * COLS + col] = x;
-            sm[jg][s] = J;  // the same from every thread of a slot
-            sl[jg][s] = L;
-        }
-        __syncthreads();
-        if (jg == 0) {
-#pragma unroll
-            for (uint32_t g = 1; g < JG; g++)
-                join(reinterpret_cast<const float4*>(so)[g * COLS + col], sm[g][s], sl[g][s]);
-        }
-    }
-    if (jg == 0) unit.write(col, x, L);
 }
 
 // W: words of codes in a quarter row (head up to 32 W). NT: four query slots each. NW: warps.
@@ -377,7 +382,6 @@ __global__ void __launch_bounds__(NW * 32, kSmWarps / NW)
     using St = Stage<W>;
     constexpr uint32_t RING = kStages * St::BYTES;  // a warp's turns
     constexpr uint32_t QF = NT * W * 2 * 32;        // operand words (uint2) of a unit's queries
-    static_assert(S <= kWarps, "a warp per slot");
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float s_m[kWarps][S], s_l[kWarps][S];
     __shared__ Slot s_slot[2][S];
@@ -529,67 +533,79 @@ __global__ void __launch_bounds__(NW * 32, kSmWarps / NW)
     };
     // Queries, times log2(e) / sqrt(head), as operand columns: column 2 (s % 4) of slot s is the
     // whole number next to q 2^e, the next one the rest; e brings the head's largest |q| to
-    // [2^10, 2^11). Warp s takes slot s, a lane four dims.
-    float qx[4];
-    int32_t qlimit = 0;
+    // [2^10, 2^11). Warp w takes slots w, w + NW, .. , a lane four dims.
+    constexpr uint32_t TAKES = (S + NW - 1) / NW;
+    float qx[TAKES][4];
+    int32_t qlimit[TAKES];
     auto read_queries = [&](const Span& span) {
-        if (warp >= S) return;
-        uint32_t row, head;
-        const bool live = Unit<W, S, OT>{p, span.item, span.kvh, span.sub}.slot(warp, &row, &head);
-        const uint32_t d0 = lane * 4, hd = p.c.head;
-        qx[0] = qx[1] = qx[2] = qx[3] = 0.0f;
-        if (live && d0 < hd) {
-            const float* src = p.q + ((uint64_t)row * p.heads + head) * hd + d0;
-            if (p.qvec) {
-                const uint4 a = ld16(src);
-                qx[0] = __uint_as_float(a.x); qx[1] = __uint_as_float(a.y);
-                qx[2] = __uint_as_float(a.z); qx[3] = __uint_as_float(a.w);
-            } else {
 #pragma unroll
-                for (uint32_t k = 0; k < 4; k++)
-                    if (d0 + k < hd) qx[k] = __uint_as_float(ld4(src + k));
+        for (uint32_t j = 0; j < TAKES; j++) {
+            const uint32_t s = warp + NW * j;
+            if (s >= S) return;
+            float(&x)[4] = qx[j];
+            uint32_t row, head;
+            const bool live =
+                Unit<W, S, OT>{p, span.item, span.kvh, span.sub}.slot(s, &row, &head);
+            const uint32_t d0 = lane * 4, hd = p.c.head;
+            x[0] = x[1] = x[2] = x[3] = 0.0f;
+            if (live && d0 < hd) {
+                const float* src = p.q + ((uint64_t)row * p.heads + head) * hd + d0;
+                if (p.qvec) {
+                    const uint4 a = ld16(src);
+                    x[0] = __uint_as_float(a.x); x[1] = __uint_as_float(a.y);
+                    x[2] = __uint_as_float(a.z); x[3] = __uint_as_float(a.w);
+                } else {
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; k++)
+                        if (d0 + k < hd) x[k] = __uint_as_float(ld4(src + k));
+                }
             }
+            // past the last slot: nothing of it is written
+            qlimit[j] = live ? (int32_t)min(p.step[row].position, 0x7fffffffu) : 0x7fffffff;
+            if (live && qlimit[j] >= (int32_t)p.c.seq) qlimit[j] = -1;
         }
-        // past the last slot: nothing of it is written
-        qlimit = live ? (int32_t)min(p.step[row].position, 0x7fffffffu) : 0x7fffffff;
-        if (live && qlimit >= (int32_t)p.c.seq) qlimit = -1;
     };
     auto set_queries = [&](uint2* qf, Slot* slots) {
-        if (warp >= S) return;
         const float unit_scale = kLog2e / sqrtf((float)p.c.head);
-        float top = 0.0f, sum = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            qx[k] *= unit_scale;
-            top = fmaxf(top, fabsf(qx[k]));
-            sum += qx[k];
-        }
-        top = warp_max(top);
-        int e = 10 - ((int)(__float_as_uint(top) >> 23) - 127);
-        e = min(max(e, -100), 100);
-        const float up = __uint_as_float((uint32_t)(e + 127) << 23);
-        float first = 0.0f, rest = 0.0f;
-        const uint32_t word = lane / 2, col = 2 * (warp % 4);
-        __half* dst = reinterpret_cast<__half*>(qf) + lane % 2;
+        for (uint32_t j = 0; j < TAKES; j++) {
+            const uint32_t s = warp + NW * j;
+            if (s >= S) return;
+            float(&x)[4] = qx[j];
+            float top = 0.0f, sum = 0.0f;
 #pragma unroll
-        for (uint32_t k = 0; k < 4; k++) {
-            const float v = qx[k] * up, w = rintf(v);  // the rest is NaN where q is not finite
-            first += w;
-            rest += v - w;
-            if (word < 4 * W) {
-                // code k of a half word is at bits 4 k: even k as c 2^-24, odd as 16 c 2^-24
-                const uint32_t at = (((warp / 4) * W + word % W) * 2 + k / 2) * 32 + word / W;
-                const float f = k % 2 ? 0.0625f : 1.0f;
-                dst[((at + col * 4) * 2 + k % 2) * 2] = __float2half_rn(w * f);
-                dst[((at + col * 4 + 4) * 2 + k % 2) * 2] = __float2half_rn((v - w) * f);
+            for (int k = 0; k < 4; k++) {
+                x[k] *= unit_scale;
+                top = fmaxf(top, fabsf(x[k]));
+                sum += x[k];
             }
+            top = warp_max(top);
+            int e = 10 - ((int)(__float_as_uint(top) >> 23) - 127);
+            e = min(max(e, -100), 100);
+            const float up = __uint_as_float((uint32_t)(e + 127) << 23);
+            float first = 0.0f, rest = 0.0f;
+            const uint32_t word = lane / 2, col = 2 * (s % 4);
+            __half* dst = reinterpret_cast<__half*>(qf) + lane % 2;
+#pragma unroll
+            for (uint32_t k = 0; k < 4; k++) {
+                const float v = x[k] * up, w = rintf(v);  // the rest is NaN where q is not finite
+                first += w;
+                rest += v - w;
+                if (word < 4 * W) {
+                    // code k of a half word is at bits 4 k: even k as c 2^-24, odd as 16 c 2^-24
+                    const uint32_t at = (((s / 4) * W + word % W) * 2 + k / 2) * 32 + word / W;
+                    const float f = k % 2 ? 0.0625f : 1.0f;
+                    dst[((at + col * 4) * 2 + k % 2) * 2] = __float2half_rn(w * f);
+                    dst[((at + col * 4 + 4) * 2 + k % 2) * 2] = __float2half_rn((v - w) * f);
+                }
+            }
+            sum = warp_sum(sum);
+            first = warp_sum(first);
+            rest = warp_sum(rest);
+            if (lane == 0)
+                slots[s] = Slot{16777216.0f / up, sum, first * (-8.0f / 16777216.0f),
+                                rest * (-8.0f / 16777216.0f), qlimit[j]};
         }
-        sum = warp_sum(sum);
-        first = warp_sum(first);
-        rest = warp_sum(rest);
-        if (lane == 0)
-            slots[warp] = Slot{16777216.0f / up, sum, first * (-8.0f / 16777216.0f),
-                               rest * (-8.0f / 16777216.0f), qlimit};
     };
 
     if (warp == 0) plan(begin, s_span[0]);
@@ -918,13 +934,23 @@ void record_width(ab_scheme* s, const char* label, Kv4AttnParams p, int32_t out_
     const uint32_t blocks = (uint32_t)((slots + S - 1) / S);
     p.items = p.shared ? blocks : p.rows;
     p.per_item = p.c.kv_heads * (p.shared ? 1 : blocks);
-    const bool f32 = out_dtype == AB_F32;
-    if (S == 8)
-        f32 ? record_one<W, 2, 8, float>(s, label, p) : record_one<W, 2, 8, bf16>(s, label, p);
-    else if ((uint64_t)p.items * p.per_item > (uint64_t)s->rt->sm_count * (kSmWarps / 4))
-        f32 ? record_one<W, 1, 4, float>(s, label, p) : record_one<W, 1, 4, bf16>(s, label, p);
-    else
-        f32 ? record_one<W, 1, 8, float>(s, label, p) : record_one<W, 1, 8, bf16>(s, label, p);
+    const bool many = (uint64_t)p.items * p.per_item > (uint64_t)s->rt->sm_count * (kSmWarps / 4);
+    auto record = [&](auto nt, auto nw) {
+        constexpr int NT = decltype(nt)::value, NW = decltype(nw)::value;
+        if (out_dtype == AB_F32) record_one<W, NT, NW, float>(s, label, p);
+        else record_one<W, NT, NW, bf16>(s, label, p);
+    };
+    constexpr std::integral_constant<int, 1> one;
+    constexpr std::integral_constant<int, 2> two;
+    constexpr std::integral_constant<int, 4> four;
+    constexpr std::integral_constant<int, 8> eight;
+    if (S == 4) {
+        many ? record(one, four) : record(one, eight);
+    } else if constexpr (W < 4) {
+        many ? record(two, four) : record(two, eight);
+    } else {
+        record(two, eight);
+    }
 }
 
 }  // namespace

@@ -230,6 +230,7 @@ def test_offsets_past_32_bits(rt):
 
 
 @pytest.mark.parametrize("heads,kv,head,out_dtype", [(4, 1, 128, ab.BF16), (4, 2, 33, ab.F32),
+                                                     (8, 1, 128, ab.F32), (6, 1, 90, ab.BF16),
                                                      (3, 1, 96, ab.F32), (2, 2, 20, ab.BF16)])
 def test_attention_of_many_short_rows(rt, heads, kv, head, out_dtype):
     """More units of up to four query heads than the device holds small blocks; lengths about the
