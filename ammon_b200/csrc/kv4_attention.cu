@@ -642,7 +642,7 @@ __global__ void __launch_bounds__(NW * 32, kSmWarps / NW)
         // Weights are w = 2^(score - M). M is the largest score + log2 step of V so far, less TOP,
         // moved when a w x step reaches 2^11: as for the queries, its whole number is one operand
         // column, exact in the sums, and the rest, 11 bits of at most a half, the other. With TOP 9
-        // f32 outputs of 100 positions were up to 1.1e-6 off, with 10 6e-7.
+        // f32 outputs of 100 positions were up to 1.1e-6 off, with 10 some 6e-7 on the same inputs.
         constexpr float TOP = F32 ? 10.0f : 9.0f;
         float o[NT][2 * W][2], kept[NA][2 * W][4], l[NT], pm[NT], M[NT], cap[NT];
 #pragma unroll
