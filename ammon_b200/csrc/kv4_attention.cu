@@ -639,10 +639,16 @@ __global__ void __launch_bounds__(NW * 32, kSmWarps / NW)
         lowest = min(lowest, __shfl_xor_sync(0xffffffffu, lowest, 2));
 
         // ---- the positions -----------------------------------------------------------------
-        // Weights are w = 2^(score - M). M is the largest score + log2 step of V so far, less TOP,
-        // moved when a w x step reaches 2^11: as for the queries, its whole number is one operand
-        // column, exact in the sums, and the rest, 11 bits of at most a half, the other. With TOP 9
-        // f32 outputs of 100 positions were up to 1.1e-6 off, with 10 some 6e-7 on the same inputs.
+        // Weights are w = 2^(score - M). M is the largest score + log2 g so far, less TOP, moved when
+        // a w x g reaches 2^11; g is the step of V where that is not small. As for the queries, the
+        // whole number of w x step is one operand column, exact in the sums, and the rest, 11 bits
+        // of at most a half, the other. With TOP 9 f32 outputs of 100 positions were up to 1.1e-6
+        // off, with 10 some 6e-7 on the same inputs. g is at least a 2^-20th of the offset, so that
+        // 2^31 terms w x offset are below 2^63 (a step below that adds less than the offset's own
+        // rounding), and at least kLeast, so that as many weights are below 2^126. (A bound on
+        // w x step alone let the weights of vectors without a step overflow; this one costs 1 to 2%
+        // at many short units, 43.3 to 44.2 us at 256 streams, nothing at one long row.)
+        constexpr float kLeast = 0x1p-84f;
         constexpr float TOP = F32 ? 10.0f : 9.0f;
         float o[NT][2 * W][2], kept[NA][2 * W][4], l[NT], pm[NT], M[NT], cap[NT];
 #pragma unroll
@@ -696,6 +702,10 @@ __global__ void __launch_bounds__(NW * 32, kSmWarps / NW)
                     }
                 }
             }
+            float g[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                g[i] = fmaxf(fmaxf(bf16lo(vs[i]), fabsf(bf16hi(vs[i])) * 0x1p-20f), kLeast);
             // score - M = s (q . (c - 8)) + (m + 8 s) sum q - M, taken off M first: the exact
             // whole-number sum meets it inside one rounding, at the size of the difference, so a
             // large score costs the weights no digits
@@ -715,7 +725,8 @@ __global__ void __launch_bounds__(NW * 32, kSmWarps / NW)
                         w[nt][i] = ex2(sc[nt][i]);
                         ws[nt][i] = out ? 0.0f : w[nt][i] * bf16lo(vs[i]);
                     }
-                    over |= fmaxf(fmaxf(ws[nt][0], ws[nt][1]), fmaxf(ws[nt][2], ws[nt][3])) > cap[nt];
+                    over |= fmaxf(fmaxf(w[nt][0] * g[0], w[nt][1] * g[1]),
+                                  fmaxf(w[nt][2] * g[2], w[nt][3] * g[3])) > cap[nt];
                 }
             };
             const bool masked = (int32_t)(t + kTurn - 1) > lowest;
@@ -727,9 +738,8 @@ __global__ void __launch_bounds__(NW * 32, kSmWarps / NW)
                     float top = -INFINITY;
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        // a step below 2^-90 counts as that: its weight must stay finite
-                        const int e = (int)(vs[i] << 16 >> 23) - 127;
-                        top = fmaxf(top, sc[nt][i] + (float)max(e, -90));
+                        const int e = (int)(__float_as_uint(g[i]) >> 23) - 127;
+                        top = fmaxf(top, sc[nt][i] + (float)e);
                     }
 #pragma unroll
                     for (int x = 4; x < 32; x <<= 1)
