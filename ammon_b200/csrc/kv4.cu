@@ -296,7 +296,8 @@ __global__ void __launch_bounds__(kThreads, 6)
     uint32_t word[2] = {0, 0};
     if (!bad && s > 0.0f) {
         const float inv = 1.0f / (15.0f * s);
-        bool exactly = s < 0x1p-100f;
+        // where 15 s or its reciprocal leaves the normal numbers
+        bool exactly = s < 0x1p-100f || s > 0x1p120f;
         if constexpr (sizeof(T) == 2) {
             const float q = -m * inv, twice = fmaf(q, 30.0f, kMagic) - kMagic;
             exactly |= (q > 0.0f && q < 1.1f && fmaf(0.5f * twice, s, m) == 0.0f &&
