@@ -164,6 +164,8 @@ def _empty_cache(lead, kv, seq, head):
 
 
 def prepare(case, seed):
+    if own:
+        _on_the_runtimes_stream()
     gen = torch.Generator(device=DEVICE).manual_seed(seed)
     kv, head, seq = case["kv"], case["head"], case["seq"]
     state = {"case": dict(case)}
@@ -312,13 +314,25 @@ def _plain_attend(state):
 
 
 # ---- the framework's calls --------------------------------------------------------------------
-def _record(state):
+def _on_the_runtimes_stream():
+    """The runtime works on a stream of its own, with which nothing orders torch's: a program that
+    mixes the two has torch work there too."""
     import ammon_b200 as ab
-    from ammon_b200 import kernels as K
 
     global _runtime
     if _runtime is None:
         _runtime = ab.create_runtime(torch.cuda.current_device())
+    before = torch.cuda.current_stream()
+    if before.cuda_stream != _runtime.stream:
+        stream = torch.cuda.ExternalStream(_runtime.stream)
+        stream.wait_stream(before)
+        torch.cuda.set_stream(stream)
+
+
+def _record(state):
+    import ammon_b200 as ab
+    from ammon_b200 import kernels as K
+
     rt, case = _runtime, state["case"]
     scheme = rt.scheme()
     t = {n: ab.Tensor.from_torch(x, rt) for n, x in state.items() if isinstance(x, torch.Tensor)}
