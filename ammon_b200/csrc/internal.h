@@ -94,6 +94,7 @@ struct Runtime {
     int device = 0;
     int sm_count = 0;
     cudaStream_t stream = nullptr;
+    cudaStream_t clears = nullptr;  // clear_device's
     // device flag block (256 bytes): [0] u32 bit flags raised by kernels, [8] u64 limit of
     // every bounded wait in nanoseconds (read by the kernels once a wait has lasted 1 ms)
     uint32_t* flags = nullptr;
@@ -103,12 +104,13 @@ struct Runtime {
     void set_wait_limit_ms(uint64_t ms);  // writes the limit into the flag block
 };
 
-// Zeroes device memory before anything recorded or copied on the runtime's stream can reach it.
-// (A plain cudaMemset runs on the default stream, which the runtime's does not wait for: it could
-// clear memory that a copy or a kernel on the runtime's stream had already filled.)
+// Zeroes device memory, done when it returns: the runtime's stream, other streams and blocking
+// copies may use the memory at once. The clear has a stream of its own, so work that is queued on
+// the runtime's stream is not waited for. (A plain cudaMemset runs on the default stream, which the
+// runtime's does not wait for: it could clear memory that a copy or a kernel there had filled.)
 inline cudaError_t clear_device(const Runtime* rt, void* p, size_t bytes) {
-    const cudaError_t e = cudaMemsetAsync(p, 0, bytes, rt->stream);
-    return e == cudaSuccess ? cudaStreamSynchronize(rt->stream) : e;
+    const cudaError_t e = cudaMemsetAsync(p, 0, bytes, rt->clears);
+    return e == cudaSuccess ? cudaStreamSynchronize(rt->clears) : e;
 }
 
 enum DeviceFlag : uint32_t {

@@ -256,6 +256,8 @@ int ab_runtime_create(int32_t device, ab_runtime** out) {
                        "query SM count");
             cuda_check(cudaStreamCreateWithFlags(&rt->stream, cudaStreamNonBlocking),
                        "create stream");
+            cuda_check(cudaStreamCreateWithFlags(&rt->clears, cudaStreamNonBlocking),
+                       "create stream");
             cuda_check(cudaMalloc(&rt->flags, 256), "allocate flag word");
             cuda_check(cudaMemset(rt->flags, 0, 256), "clear flag word");
             uint64_t limit_ms = 2000;
@@ -266,6 +268,7 @@ int ab_runtime_create(int32_t device, ab_runtime** out) {
             rt->set_wait_limit_ms(limit_ms);
         } catch (...) {
             if (rt->stream) cudaStreamDestroy(rt->stream);
+            if (rt->clears) cudaStreamDestroy(rt->clears);
             if (rt->flags) cudaFree(rt->flags);
             delete rt;
             throw;
@@ -280,6 +283,7 @@ int ab_runtime_destroy(ab_runtime* rt) {
         rt->activate();
         cudaStreamSynchronize(rt->stream);
         cudaStreamDestroy(rt->stream);
+        cudaStreamDestroy(rt->clears);
         cudaFree(rt->flags);
         delete rt;
     });
