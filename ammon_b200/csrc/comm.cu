@@ -150,9 +150,9 @@ bool comm_peers_setup(ab_comm* c, size_t max_elems) {
     std::memset(&mine, 0, sizeof(mine));
     int ok = 0;
     if (want && cudaMalloc(&c->local, bytes) == cudaSuccess &&
-        cudaMemset(c->local, 0, bytes) == cudaSuccess &&
+        clear_device(c->rt, c->local, bytes) == cudaSuccess &&
         cudaMalloc(&c->epoch, sizeof(uint64_t)) == cudaSuccess &&
-        cudaMemset(c->epoch, 0, sizeof(uint64_t)) == cudaSuccess &&
+        clear_device(c->rt, c->epoch, sizeof(uint64_t)) == cudaSuccess &&
         cudaIpcGetMemHandle(&mine, c->local) == cudaSuccess)
         ok = 1;
     cudaGetLastError();
@@ -219,7 +219,7 @@ bool comm_fused_block(ab_comm* c, size_t bytes, unsigned char** local,
         std::memset(&mine, 0, sizeof(mine));
         int ok = 0;
         if (cudaMalloc(&c->fused_local, bytes) == cudaSuccess &&
-            cudaMemset(c->fused_local, 0, bytes) == cudaSuccess &&
+            clear_device(c->rt, c->fused_local, bytes) == cudaSuccess &&
             cudaIpcGetMemHandle(&mine, c->fused_local) == cudaSuccess)
             ok = 1;
         cudaGetLastError();
@@ -583,7 +583,7 @@ int ab_comm_loopback_reduce(ab_runtime* rt, uint32_t world, uint32_t ready, uint
         // one float4 of every rank per thread: all of a batched step's peer loads in flight at
     // once (up to 64 rows x 4096 = 256 CTAs); a batch-1 row takes 4 CTAs
     const unsigned grid = std::max(1u, std::min(512u, (n + 1023) / 1024));
-        cudaError_t e = cudaMemset(d, 0, bytes);
+        cudaError_t e = clear_device(rt, d, bytes);
         if (e == cudaSuccess) e = cudaMemcpy(d, head.data(), head.size() * 8, cudaMemcpyHostToDevice);
         if (e == cudaSuccess)
             e = cudaMemcpy(slots, h.data(), h.size() * 4, cudaMemcpyHostToDevice);

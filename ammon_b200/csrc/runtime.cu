@@ -259,7 +259,7 @@ int ab_runtime_create(int32_t device, ab_runtime** out) {
             cuda_check(cudaStreamCreateWithFlags(&rt->clears, cudaStreamNonBlocking),
                        "create stream");
             cuda_check(cudaMalloc(&rt->flags, 256), "allocate flag word");
-            cuda_check(cudaMemset(rt->flags, 0, 256), "clear flag word");
+            cuda_check(clear_device(rt, rt->flags, 256), "clear flag word");
             uint64_t limit_ms = 2000;
             if (const char* e = std::getenv("AMMON_B200_WAIT_MS")) {
                 const long v = std::atol(e);
