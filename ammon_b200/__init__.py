@@ -81,6 +81,14 @@ class Runtime:
     def stream(self) -> int:
         return int(_abi.lib().ab_runtime_stream(self._h) or 0)
 
+    def torch_stream(self):
+        """The runtime's stream as torch's: what torch does under ``with
+        torch.cuda.stream(rt.torch_stream())`` is ordered with what the runtime does. Nothing
+        orders the runtime's work with any other stream of torch's."""
+        import torch
+
+        return torch.cuda.ExternalStream(self.stream, device=self.device)
+
     @property
     def sm_count(self) -> int:
         n = C.c_int32()
@@ -171,6 +179,8 @@ class Tensor:
 
     @classmethod
     def from_torch(cls, tensor, rt: Optional[Runtime] = None) -> "Tensor":
+        """The tensor's memory, not a copy. Torch's work on it has to be ordered with the
+        runtime's: run it on ``rt.torch_stream()``, or let the streams wait for each other."""
         import torch
 
         if not tensor.is_contiguous():
