@@ -21,8 +21,8 @@
 // unpacking gives (0 4 1 5 2 6 3 7): Q's dims are staged in the same order, O's put right when
 // they are written.
 //
-// Few blocks split their tiles over several (as many as the device holds at once); the last one
-// to finish a slot block joins the parts in order.
+// Few blocks split their tiles over several (as many as the device holds at once), and no block
+// takes more than kMaxTiles; the last one to finish a slot block joins the parts in order.
 // Measured, 8 kv heads of 4 query heads, head 128: 256 rows over 2048 positions 35.5 us (the
 // mma.sync kernel of kv4_attention.cu takes 80), 1024 over 8192 346 us (867), of which a tile is
 // some 2.5 us: the weights' arithmetic, 16384 exponentials and the scales' broadcast reads, in
@@ -59,6 +59,9 @@ constexpr uint32_t kThreads = kSoftmax + kUnpack + 32;
 // Columns of TMEM: S twice, each replaced by its P (value, rest), O, Q (value, rest).
 constexpr uint32_t kTmemCols = 512, kTmemO = 256, kTmemQ = 384;
 constexpr uint32_t kMinTiles = 2;    // a part has at least so many
+// and at most these: the tensor unit's additions cut off, so a long chain of them sinks (sums of
+// equal codes 2.9e-4 low over 131072 positions, 2.9e-3 over 1000000)
+constexpr uint32_t kMaxTiles = 1024;
 constexpr float kRescale = 11.5f;    // base 2: P stays below 2^kRescale steps of V
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -66,7 +69,8 @@ struct PromptParams {
     const float* q;  // [rows, heads, head]
     bf16* out;       // [rows, heads * head]
     Kv4View c;
-    uint32_t rows, heads, group, splits;
+    uint32_t rows, heads, group;
+    uint32_t splits, even;  // parts of a slot block at most, and without kMaxTiles
     int qvec, ovec;  // 16-byte accesses of q and out
     float* part;     // [slot block, kv head, split][HD + 2][128]
     uint32_t* tickets;
@@ -77,7 +81,7 @@ struct PromptParams {
 template <int HD>
 struct Layout {
     static constexpr uint32_t T = kTile * HD * 2;  // K or V of a tile
-    static constexpr uint32_t SCALES_AT = kStages * 2 * T;  // [stage][K, V][s, m'][64]
+    static constexpr uint32_t SCALES_AT = kStages * 2 * T;  // [stage][K, V][s, m'][kTile]
     static constexpr uint32_t RED_AT = SCALES_AT + kStages * 4 * kTile * 4;
     // maxima [2 tiles][kShare][128]; sums of q, of weights, of weights x m' [kShare][128]
     static constexpr uint32_t BYTES = RED_AT + 5 * kShare * kRows * 4;
@@ -208,6 +212,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t kvh = blockIdx.y, slot = blockIdx.x * kRows + tid % kRows;
 
     pdl_wait();
+    if (blockIdx.z >= p.even) {  // these parts exist where the others are full
+        bool some = false;
+        if (tid < kRows && slot / p.group < p.rows) {
+            const uint32_t pos = p.step[slot / p.group].position;
+            some = pos < p.c.seq && pos / (kTile * kMaxTiles) >= blockIdx.z;
+        }
+        if (!__syncthreads_or(some)) return;
+    }
     // The queries, for now in the room of the later stages: whole rows a few lanes each (a row a
     // thread, read where it is used, took 3 us).
     float* staged = reinterpret_cast<float*>(smem + 2 * LY::T);
@@ -250,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t until = max(max(s_most[0], s_most[1]), max(s_most[2], s_most[3]));
     // the block's share of the tiles
     const uint32_t all = (until + kTile - 1) / kTile;
-    const uint32_t each = max(kMinTiles, (all + p.splits - 1) / p.splits);
+    const uint32_t each = min(kMaxTiles, max(kMinTiles, (all + p.even - 1) / p.even));
     const uint32_t parts = max(1u, (all + each - 1) / each);
     if (blockIdx.z >= parts) return;
     const uint32_t t_lo = blockIdx.z * each;
@@ -656,7 +668,9 @@ void record_one(ab_scheme* s, const char* label, PromptParams p) {
     static_assert(smem + 512 <= 227 * 1024);
     const uint64_t blocks = ((uint64_t)p.rows * p.group + kRows - 1) / kRows;
     const uint64_t units = blocks * p.c.kv_heads;
-    p.splits = (uint32_t)std::max<uint64_t>(1, s->rt->sm_count / units);
+    const uint32_t longest = (uint32_t)(((uint64_t)p.c.seq + kTile * kMaxTiles - 1) / (kTile * kMaxTiles));
+    p.even = (uint32_t)std::max<uint64_t>(1, s->rt->sm_count / units);
+    p.splits = std::max(p.even, longest);
     s->rt->activate();
     cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
                "kv4_attention shared memory");
