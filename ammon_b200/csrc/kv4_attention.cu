@@ -11,18 +11,19 @@
 // aligns products by their exponent fields, so subnormals lose low bits of a long factor; the
 // other operand is therefore a whole number of at most 11 bits, whose products and sums are exact
 // (with an fp16 value there, f32 results were 7e-5 off instead of some 1e-7). The cache
-// is the 16-row operand (16 positions for K, 16 dims for V), read once for all query heads of
-// its group; the queries and the weights are the 8-column one, each head taking two columns of
+// is the 16-row operand (16 positions for K, 16 dims for V), read once for up to eight query heads
+// of its group (more are units of their own); the queries and the weights are the 8-column one, each head taking two columns of
 // fp16, the whole number and the rest, together 22 bits. So f32 results keep their digits, and one
 // lane's accumulators all belong to one head: its maximum, sum and rescaling need no exchange.
 //
-// Bound: the packed bytes, and before them the instructions: a warp's 32 positions (head 128) are
-// 4352 bytes and about 470 instructions, 32 of them mma. Each warp keeps the next 32 positions on
-// their way into shared memory while it computes on the present ones. Measured (8 kv heads of 4
-// query heads, head 128): one row of 131072 positions 36.3 us (143 MB, 3.9 TB/s, half the issue
-// slots used); 64 rows of 1 to 8192, 56 us (265 MB, 4.7 TB/s); one of 8001, 10.3 us. 256 rows of 1 to
-// 1024 positions of 12 heads of 64 take 43 us (113 MB, 2.6 TB/s): five units a block, whose starts
-// and joins are what its barriers wait for.
+// Bound: latency. A warp's 32 positions (head 128) are 4352 bytes and about 490 instructions, 32 of
+// them mma. Each warp keeps the next 32 positions on their way into shared memory while it computes
+// on the present ones; registers and shared memory hold 16 warps an SM. Measured (8 kv heads of 4
+// query heads, head 128): one row of 131072 positions 36.9 us (143 MB, 3.9 TB/s, half the issue
+// slots and 0.6 of the memory's rate used: too few bytes under way, and barriers at the ends); 64
+// rows of 1 to 8192, 56.5 us (265 MB, 4.7 TB/s); one of 8001, 10.2 us. 256 rows of 1 to 1024
+// positions of 12 heads of 64 take 44 us (113 MB, 2.6 TB/s): five units a block, whose starts and
+// joins are what its barriers wait for.
 //
 // Split: the tiles (a turn of all warps of a block) of all units (a row's or a slot block's
 // positions of one kv head) form one line that the blocks of one wave share equally, so rows of
@@ -377,7 +378,7 @@ __global__ void __launch_bounds__(NW * 32, kSmWarps / NW)
     // Sums of bf16 outputs stay in the unit's accumulators. Those of f32 outputs start from zero
     // every turn and are added to running ones, the rest's with the whole numbers', outside: the
     // unit's own addition cuts off, and over a chain of positive terms that shows (5e-6 over 9
-    // turns, 1.4e-5 over 28).
+    // turns, 1.4e-5 over 28, 2.4e-4 over 1953, the 500000 positions of a block).
     constexpr bool KEEP = !F32;
     using St = Stage<W>;
     constexpr uint32_t RING = kStages * St::BYTES;  // a warp's turns

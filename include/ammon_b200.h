@@ -206,8 +206,9 @@ int ab_kvcache_destroy(ab_kvcache* c);
  * held as 4-bit codes c_i and one word with two bf16 numbers, the step s (low half) and the
  * offset m (high half), and stands for the values m + s c_i:
  *     m = bf16(min x), s = bf16(max(max x - m, 0) / 15), c_i = (x_i - m) / s to the nearest
- *     whole number (halves to even) within 0..15; all c_i are 0 where s is 0.
- * A vector that holds an infinity or NaN, or whose range overflows, is NaN throughout.
+ *     whole number (halves to even, decided in real arithmetic) within 0..15; all c_i are 0
+ *     where s is 0, and an m of zero has either sign.
+ * A vector that holds an infinity or NaN, or whose range or offset overflows, is NaN throughout.
  * Codes are AB_U32 [kv_heads, seq, words] or [batch, kv_heads, seq, words], words =
  * 4 * ceil(head / 32), 16-byte aligned: element i is bits 4 (i % 8) and up of word i / 8, the
  * elements past head are 0. Scales are AB_U32 with the same dims but the last. head is 1..128.
@@ -241,7 +242,8 @@ int ab_kernel_kv4_load(ab_scheme* s, const ab_kv4_layer* cache, ab_tensor step, 
  * any whole number of query heads per kv head. With a batch dim each row has a cache of its
  * own; without one all rows attend over the same cache, each up to its own position (the rows
  * of a prompt). A row at a position >= seq gives zeros and raises AB_ERR_DEVICE. Positions
- * past a row's own are never used, whatever they hold. out must not overlap q. Scratch is
+ * past a row's own are never used, whatever they hold. Sums are f32: results are finite where the
+ * positions times the largest |m + s c| stay below 2^116. out must not overlap q. Scratch is
  * allocated here and owned by the scheme, which therefore needs a runtime. */
 int ab_kernel_kv4_attention(ab_scheme* s, ab_tensor q, const ab_kv4_layer* cache, ab_tensor out,
                             ab_tensor step);
